@@ -27,6 +27,10 @@ setup(
                      "-U__CUDA_NO_BFLOAT16_CONVERSIONS__", "-U__CUDA_NO_HALF2_OPERATORS__"],
         },
         libraries=["cuda"],
+        # torch throws and catches through the shared C++ runtime: an extension linked with the
+        # static one (a compiler that has no usable libstdc++.so does so) crashes on its first
+        # failed argument check
+        extra_link_args=["-l:libstdc++.so.6"],
     )],
     cmdclass={"build_ext": BuildExtension.with_options(use_ninja=True)},
 )
