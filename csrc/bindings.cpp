@@ -128,6 +128,21 @@ void dit_qk_rope(torch::Tensor qkv, c10::optional<torch::Tensor> qw, c10::option
 void gemm_q(torch::Tensor A, torch::Tensor Wq, int64_t type, int64_t K, torch::Tensor C, int64_t epi,
             torch::Tensor err);
 
+void kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tensor vc, torch::Tensor ks,
+                torch::Tensor vs, torch::Tensor kt, torch::Tensor vt, int64_t slot, int64_t p0);
+void kv8_read(torch::Tensor kc, torch::Tensor vc, torch::Tensor ks, torch::Tensor vs, torch::Tensor kt,
+              torch::Tensor vt, int64_t slot, int64_t length, int64_t start, torch::Tensor k_out,
+              torch::Tensor v_out);
+torch::Tensor kv8_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+void attn_decode_kv8(torch::Tensor proj, c10::optional<torch::Tensor> q_norm_w, c10::optional<torch::Tensor> k_norm_w,
+                     torch::Tensor inv_freq, torch::Tensor kc, torch::Tensor vc, torch::Tensor ks, torch::Tensor vs,
+                     torch::Tensor kt, torch::Tensor vt, torch::Tensor slots, torch::Tensor pos, torch::Tensor ws,
+                     torch::Tensor out, int64_t Hq, int64_t rot, bool gated, double eps,
+                     c10::optional<torch::Tensor> rope_delta);
+void attn_prefill_kv8(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torch::Tensor ks, torch::Tensor vs,
+                      torch::Tensor kt, torch::Tensor vt, int64_t slot, int64_t p0, torch::Tensor out, int64_t Hq,
+                      double scale, c10::optional<torch::Tensor> gate, int64_t gate_head_stride, torch::Tensor err);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_pdl", [](bool on) { hx_pdl_enabled() = on; });
   m.def("gemv", &gemv);
@@ -174,6 +189,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_prefill_tc", &attn_prefill_tc, py::arg("q"), py::arg("kc"), py::arg("vc"), py::arg("out"), py::arg("Hq"),
         py::arg("p0"), py::arg("scale"), py::arg("gate"), py::arg("gate_head_stride"), py::arg("err"),
         py::arg("causal") = true);
+  m.def("kv8_append", &kv8_append, py::arg("k"), py::arg("v"), py::arg("kc"), py::arg("vc"), py::arg("ks"),
+        py::arg("vs"), py::arg("kt"), py::arg("vt"), py::arg("slot"), py::arg("p0"));
+  m.def("kv8_read", &kv8_read, py::arg("kc"), py::arg("vc"), py::arg("ks"), py::arg("vs"), py::arg("kt"),
+        py::arg("vt"), py::arg("slot"), py::arg("length"), py::arg("start"), py::arg("k_out"), py::arg("v_out"));
+  m.def("kv8_workspace", &kv8_workspace, py::arg("B"), py::arg("Hq"), py::arg("Hkv"), py::arg("D"));
+  m.def("attn_decode_kv8", &attn_decode_kv8, py::arg("proj"), py::arg("q_norm_w"), py::arg("k_norm_w"),
+        py::arg("inv_freq"), py::arg("kc"), py::arg("vc"), py::arg("ks"), py::arg("vs"), py::arg("kt"), py::arg("vt"),
+        py::arg("slots"), py::arg("pos"), py::arg("ws"), py::arg("out"), py::arg("Hq"), py::arg("rot"),
+        py::arg("gated"), py::arg("eps"), py::arg("rope_delta") = py::none());
+  m.def("attn_prefill_kv8", &attn_prefill_kv8, py::arg("q"), py::arg("kc"), py::arg("vc"), py::arg("ks"),
+        py::arg("vs"), py::arg("kt"), py::arg("vt"), py::arg("slot"), py::arg("p0"), py::arg("out"), py::arg("Hq"),
+        py::arg("scale"), py::arg("gate"), py::arg("gate_head_stride"), py::arg("err"));
   m.def("sample_step", &sample_step);
   m.def("moe_fused", &moe_fused, py::arg("x"), py::arg("norm_w"), py::arg("eps"), py::arg("router"), py::arg("w_gu"),
         py::arg("w_d"), py::arg("E"), py::arg("topk"), py::arg("has_shared"), py::arg("norm_topk"),

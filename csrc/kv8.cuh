@@ -1,0 +1,74 @@
+// The 8-bit KV cache of one layer: layout, codes and the device helpers its kernels share.
+//
+// Tokens are held in blocks of 32. A complete block of one slot and kv head has 8-bit codes
+// (int8 or e4m3) and one f32 scale for K and one for V:
+//   a = max |x| over the block's finite values, scale = a / M, code = rne(x * (M / a)),
+//   value = code * scale,  M = 127 (int8) or 448 (e4m3).
+// A block whose a is below 1e-30 gets scale 0 and codes 0; an infinity becomes the largest
+// code and a NaN code 0 (neither can be told apart once it is held in 8 bits).
+// The sequence's last block is also held in bf16, the tail, and is read from there until it
+// is complete. What the cache holds so depends on the tokens alone, not on whether they came
+// one at a time or as a prompt, and no code is ever quantised a second time.
+//
+//   kc  [S, Hkv, NB, D/64, 32 keys, 64 dims]     vc  [S, Hkv, NB, D/64, 64 dims, 32 keys]
+//   ks, vs  f32 [S, Hkv, NB]
+//   kt  bf16 [S, Hkv, D/64, 32, 64]              vt  bf16 [S, Hkv, D/64, 64, 32]
+// Blocks are sets of contiguous 2 KB panels whose rows run along the dimension that Q K^T
+// (dims) and P V (keys) sum over, so both products read their operand as it is stored.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "kv8_args.h"
+
+namespace hx {
+
+constexpr float kKV8Least = 1e-30f;                 // a block below this holds zeros
+
+// Codes by format: int8 (FP8 = false) or e4m3 (FP8 = true).
+template <bool FP8>
+HX_DEVICE float kv8_top() { return FP8 ? 448.f : 127.f; }
+
+template <bool FP8>
+HX_DEVICE uint8_t kv8_code(float x, float inv) {
+  const float y = x * inv;
+  if constexpr (FP8) {
+    return y != y ? (uint8_t)0 : (uint8_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+  } else {
+    const int c = y != y ? 0 : __float2int_rn(fminf(fmaxf(y, -127.f), 127.f));
+    return (uint8_t)(int8_t)c;
+  }
+}
+
+template <bool FP8>
+HX_DEVICE float kv8_float(uint8_t c) {
+  if constexpr (FP8) return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+  else return (float)(int8_t)c;
+}
+
+// |x| for the block maximum: infinities and NaN do not count.
+HX_DEVICE float kv8_mag(float x) {
+  const float a = fabsf(x);
+  return a <= 3.4028235e38f ? a : 0.f;
+}
+template <bool FP8>
+HX_DEVICE float kv8_inv(float a) { return a < kKV8Least ? 0.f : kv8_top<FP8>() / a; }
+template <bool FP8>
+HX_DEVICE float kv8_scale(float a) { return a < kKV8Least ? 0.f : a / kv8_top<FP8>(); }
+
+// Calls f(integral_constant<head dim>, true_type for e4m3 or false_type for int8).
+template <typename F>
+inline void kv8_dispatch(int D, bool fp8, F&& f) {
+  auto by_fmt = [&](auto d) {
+    if (fp8) f(d, std::true_type{});
+    else f(d, std::false_type{});
+  };
+  if (D == 64) by_fmt(std::integral_constant<int, 64>{});
+  else if (D == 128) by_fmt(std::integral_constant<int, 128>{});
+  else by_fmt(std::integral_constant<int, 256>{});
+}
+
+}  // namespace hx

@@ -1,0 +1,218 @@
+// Entry points of the 8-bit KV cache (kv8.cuh): argument checks, then the launchers.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <cmath>
+
+#include "kv8_args.h"
+
+using namespace hx;
+
+#define HX_KV8_LAUNCH(expr)                                                                      \
+  do {                                                                                           \
+    const cudaError_t e_ = (expr);                                                               \
+    TORCH_CHECK(e_ == cudaSuccess, "CUDA error ", cudaGetErrorString(e_), " in " #expr);         \
+  } while (0)
+
+static bool kv8_is_fp8(const torch::Tensor& kc) { return kc.scalar_type() == at::kFloat8_e4m3fn; }
+
+static KV8 kv8_args(const torch::Tensor& kc, const torch::Tensor& vc, const torch::Tensor& ks, const torch::Tensor& vs,
+                    const torch::Tensor& kt, const torch::Tensor& vt) {
+  TORCH_CHECK(kc.is_cuda() && kc.dim() == 6 && kc.size(4) == kKV8Block && kc.size(5) == 64 && kc.is_contiguous(),
+              "kc [S, Hkv, NB, D/64, 32, 64] contiguous on the GPU");
+  TORCH_CHECK(kc.scalar_type() == at::kChar || kv8_is_fp8(kc), "cache codes are int8 or float8_e4m3fn");
+  const int64_t S = kc.size(0), H = kc.size(1), nb = kc.size(2), n = kc.size(3);
+  TORCH_CHECK(n == 1 || n == 2 || n == 4, "head dim 64, 128 or 256");
+  TORCH_CHECK(S >= 1 && H >= 1 && nb >= 1 && nb <= (1 << 24), "empty cache, or more than 2^29 tokens");
+  TORCH_CHECK(vc.scalar_type() == kc.scalar_type() && vc.is_contiguous() && vc.sizes() == at::IntArrayRef({S, H, nb, n, 64, kKV8Block}),
+              "vc [S, Hkv, NB, D/64, 64, 32] like kc");
+  for (const auto& t : {ks, vs})
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.is_contiguous() && t.sizes() == at::IntArrayRef({S, H, nb}),
+                "ks / vs f32 [S, Hkv, NB]");
+  TORCH_CHECK(kt.scalar_type() == at::kBFloat16 && kt.is_contiguous() && kt.sizes() == at::IntArrayRef({S, H, n, kKV8Block, 64}),
+              "kt bf16 [S, Hkv, D/64, 32, 64]");
+  TORCH_CHECK(vt.scalar_type() == at::kBFloat16 && vt.is_contiguous() && vt.sizes() == at::IntArrayRef({S, H, n, 64, kKV8Block}),
+              "vt bf16 [S, Hkv, D/64, 64, 32]");
+  for (const auto& t : {kc, vc, ks, vs, kt, vt})
+    TORCH_CHECK(t.device() == kc.device() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+                "cache tensors on one device, 16-byte aligned");
+  KV8 c{};
+  c.kc = reinterpret_cast<uint8_t*>(kc.data_ptr());
+  c.vc = reinterpret_cast<uint8_t*>(vc.data_ptr());
+  c.ks = ks.data_ptr<float>();
+  c.vs = vs.data_ptr<float>();
+  c.kt = reinterpret_cast<__nv_bfloat16*>(kt.data_ptr());
+  c.vt = reinterpret_cast<__nv_bfloat16*>(vt.data_ptr());
+  c.S = (int)S; c.Hkv = (int)H; c.nb = (int)nb; c.D = (int)n * 64;
+  c.fp8 = kv8_is_fp8(kc);
+  return c;
+}
+
+static void kv8_check_on(const torch::Tensor& kc, const torch::Tensor& t, const char* what) {
+  TORCH_CHECK(t.device() == kc.device(), what, " is not on the cache's device");
+}
+
+// k, v [T, Hkv, D] bf16 (any row and head stride, dims contiguous): tokens p0 .. p0+T-1 of
+// `slot`, whose tokens 0 .. p0-1 are in the cache.
+void kv8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kc, torch::Tensor vc, torch::Tensor ks,
+                torch::Tensor vs, torch::Tensor kt, torch::Tensor vt, int64_t slot, int64_t p0) {
+  KV8AppendArgs a{};
+  a.c = kv8_args(kc, vc, ks, vs, kt, vt);
+  const int64_t D = a.c.D, Hkv = a.c.Hkv;
+  for (const auto& t : {k, v}) {
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(0) == k.size(0) && t.size(1) == Hkv &&
+                    t.size(2) == D && t.stride(2) == 1,
+                "k / v [T, Hkv, D] bf16 with contiguous dims");
+    kv8_check_on(kc, t, "k / v");
+  }
+  const int64_t T = k.size(0);
+  TORCH_CHECK(slot >= 0 && slot < a.c.S, "slot ", slot, " of ", a.c.S);
+  TORCH_CHECK(p0 >= 0 && p0 + T <= (int64_t)a.c.nb * kKV8Block, "positions past the cache");
+  if (T == 0) return;
+  const c10::cuda::CUDAGuard guard(kc.device());
+  a.k = reinterpret_cast<const __nv_bfloat16*>(k.data_ptr());
+  a.v = reinterpret_cast<const __nv_bfloat16*>(v.data_ptr());
+  a.k_row = k.stride(0); a.k_head = k.stride(1);
+  a.v_row = v.stride(0); a.v_head = v.stride(1);
+  a.vec = 1;
+  for (const auto& t : {k, v})
+    if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 || (T > 1 && t.stride(0) % 8) || (Hkv > 1 && t.stride(1) % 8))
+      a.vec = 0;
+  a.slot = (int)slot; a.p0 = (int)p0; a.T = (int)T; a.b0 = (int)(p0 / kKV8Block);
+  HX_KV8_LAUNCH(kv8_append_launch(a, at::cuda::getCurrentCUDAStream()));
+}
+
+// Rows start .. start+n-1 of a slot that holds `length` tokens into k_out / v_out [Hkv, n, D]
+// bf16 (any head and row stride that keeps rows 16-byte aligned).
+void kv8_read(torch::Tensor kc, torch::Tensor vc, torch::Tensor ks, torch::Tensor vs, torch::Tensor kt,
+              torch::Tensor vt, int64_t slot, int64_t length, int64_t start, torch::Tensor k_out,
+              torch::Tensor v_out) {
+  KV8ReadArgs a{};
+  a.c = kv8_args(kc, vc, ks, vs, kt, vt);
+  const int64_t D = a.c.D, Hkv = a.c.Hkv;
+  for (const auto& t : {k_out, v_out}) {
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16 && t.dim() == 3 && t.size(0) == Hkv && t.size(1) == k_out.size(1) &&
+                    t.size(2) == D && t.stride(2) == 1,
+                "k_out / v_out [Hkv, n, D] bf16 with contiguous dims");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (Hkv == 1 || t.stride(0) % 8 == 0) &&
+                    (t.size(1) <= 1 || t.stride(1) % 8 == 0),
+                "output rows must be 16-byte aligned");
+    kv8_check_on(kc, t, "k_out / v_out");
+  }
+  const int64_t n = k_out.size(1);
+  TORCH_CHECK(slot >= 0 && slot < a.c.S, "slot ", slot, " of ", a.c.S);
+  TORCH_CHECK(length >= 0 && length <= (int64_t)a.c.nb * kKV8Block, "length past the cache");
+  TORCH_CHECK(start >= 0 && start + n <= length, "rows past the slot's ", length, " tokens");
+  if (n == 0) return;
+  const c10::cuda::CUDAGuard guard(kc.device());
+  a.k = reinterpret_cast<__nv_bfloat16*>(k_out.data_ptr());
+  a.v = reinterpret_cast<__nv_bfloat16*>(v_out.data_ptr());
+  a.k_head = k_out.stride(0); a.k_row = k_out.stride(1);
+  a.v_head = v_out.stride(0); a.v_row = v_out.stride(1);
+  a.slot = (int)slot; a.L = (int)length; a.start = (int)start; a.n = (int)n;
+  HX_KV8_LAUNCH(kv8_read_launch(a, at::cuda::getCurrentCUDAStream()));
+}
+
+// int32 scratch of attn_decode_kv8 for up to B sequences, zeroed; word 0 is its error word
+// (6001: a slot or a position outside the cache). One for each stream that decodes.
+torch::Tensor kv8_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
+  TORCH_CHECK(B >= 1 && Hkv >= 1 && Hq % Hkv == 0 && Hq >= Hkv, "batch and head counts");
+  TORCH_CHECK(D == 64 || D == 128 || D == 256, "head dim 64, 128 or 256");
+  return torch::zeros({64}, torch::TensorOptions().dtype(torch::kInt).device(torch::kCUDA));
+}
+
+void attn_decode_kv8(torch::Tensor proj, c10::optional<torch::Tensor> q_norm_w, c10::optional<torch::Tensor> k_norm_w,
+                     torch::Tensor inv_freq, torch::Tensor kc, torch::Tensor vc, torch::Tensor ks, torch::Tensor vs,
+                     torch::Tensor kt, torch::Tensor vt, torch::Tensor slots, torch::Tensor pos, torch::Tensor ws,
+                     torch::Tensor out, int64_t Hq, int64_t rot, bool gated, double eps,
+                     c10::optional<torch::Tensor> rope_delta) {
+  AttnDecodeKV8Args a{};
+  a.c = kv8_args(kc, vc, ks, vs, kt, vt);
+  const int64_t D = a.c.D, Hkv = a.c.Hkv, B = slots.numel();
+  const int64_t qw = gated ? 2 * D : D;
+  TORCH_CHECK(Hq >= Hkv && Hq % Hkv == 0, "query heads must be a multiple of the cache's ", Hkv, " kv heads");
+  TORCH_CHECK(slots.scalar_type() == at::kInt && slots.is_contiguous() && slots.dim() == 1, "slots int32 [B]");
+  TORCH_CHECK(pos.scalar_type() == at::kInt && pos.is_contiguous() && pos.numel() >= a.c.S, "pos int32 [S]");
+  TORCH_CHECK(proj.scalar_type() == at::kBFloat16 && proj.dim() == 2 && proj.size(0) == B && proj.stride(1) == 1 &&
+                  proj.size(1) >= Hq * qw + 2 * Hkv * D,
+              "proj bf16 [B, q (+ gate) | k | v]");
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.dim() == 2 && out.size(0) == B &&
+                  out.size(1) == Hq * D,
+              "out bf16 [B, Hq * D]");
+  TORCH_CHECK(rot >= 0 && rot <= D && rot % 2 == 0, "rotary dims: even, at most the head dim");
+  TORCH_CHECK(inv_freq.scalar_type() == at::kFloat && inv_freq.is_contiguous() && inv_freq.numel() >= rot / 2,
+              "inv_freq f32 [rot/2]");
+  for (const auto& w : {q_norm_w, k_norm_w})
+    if (w) {
+      TORCH_CHECK(w->scalar_type() == at::kFloat && w->is_contiguous() && w->numel() == D, "norm weights f32 [D]");
+      kv8_check_on(kc, *w, "a norm weight");
+    }
+  TORCH_CHECK(ws.scalar_type() == at::kInt && ws.is_contiguous() && ws.numel() >= 64, "ws: from kv8_workspace()");
+  kv8_check_on(kc, proj, "proj");
+  kv8_check_on(kc, inv_freq, "inv_freq");
+  kv8_check_on(kc, slots, "slots");
+  kv8_check_on(kc, pos, "pos");
+  kv8_check_on(kc, ws, "ws");
+  kv8_check_on(kc, out, "out");
+  if (rope_delta) {
+    TORCH_CHECK(rope_delta->scalar_type() == at::kInt && rope_delta->is_contiguous() && rope_delta->numel() >= a.c.S,
+                "rope_delta int32 [S]");
+    kv8_check_on(kc, *rope_delta, "rope_delta");
+    a.rope_delta = rope_delta->data_ptr<int>();
+  }
+  if (B == 0) return;
+  const c10::cuda::CUDAGuard guard(kc.device());
+  a.proj = reinterpret_cast<const __nv_bfloat16*>(proj.data_ptr());
+  a.ldp = proj.stride(0);
+  a.q_norm_w = q_norm_w ? q_norm_w->data_ptr<float>() : nullptr;
+  a.k_norm_w = k_norm_w ? k_norm_w->data_ptr<float>() : nullptr;
+  a.inv_freq = inv_freq.data_ptr<float>();
+  a.slots = slots.data_ptr<int>();
+  a.pos = pos.data_ptr<int>();
+  a.ws = ws.data_ptr<int>();
+  a.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  a.B = (int)B; a.Hq = (int)Hq; a.rot = (int)rot; a.gated = gated; a.eps = (float)eps;
+  a.sl2 = 1.4426950408889634f / sqrtf((float)D);
+  HX_KV8_LAUNCH(attn_decode_kv8_launch(a, at::cuda::getCurrentCUDAStream()));
+}
+
+// q [T, >= Hq*D] bf16 (normed, rotated); out [T, >= Hq*D] bf16; gate [T, *] bf16, head h's dims
+// at column h * gate_head_stride; err int32 [1] (bounded waits).
+void attn_prefill_kv8(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torch::Tensor ks, torch::Tensor vs,
+                      torch::Tensor kt, torch::Tensor vt, int64_t slot, int64_t p0, torch::Tensor out, int64_t Hq,
+                      double scale, c10::optional<torch::Tensor> gate, int64_t gate_head_stride, torch::Tensor err) {
+  AttnPrefillKV8Args a{};
+  a.c = kv8_args(kc, vc, ks, vs, kt, vt);
+  const int64_t D = a.c.D, Hkv = a.c.Hkv, T = q.size(0);
+  TORCH_CHECK(Hq >= Hkv && Hq % Hkv == 0, "query heads must be a multiple of the cache's ", Hkv, " kv heads");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 && q.dim() == 2 && q.stride(1) == 1 && q.size(1) >= Hq * D,
+              "q bf16 [T, Hq*D]");
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.dim() == 2 && out.size(0) == T && out.stride(1) == 1 &&
+                  out.size(1) >= Hq * D,
+              "out bf16 [T, Hq*D]");
+  TORCH_CHECK(err.scalar_type() == at::kInt && err.numel() >= 1, "err int32 [1]");
+  TORCH_CHECK(slot >= 0 && slot < a.c.S, "slot ", slot, " of ", a.c.S);
+  TORCH_CHECK(p0 >= 0 && p0 + T <= (int64_t)a.c.nb * kKV8Block, "positions past the cache");
+  kv8_check_on(kc, q, "q");
+  kv8_check_on(kc, out, "out");
+  kv8_check_on(kc, err, "err");
+  if (gate) {
+    TORCH_CHECK(gate->scalar_type() == at::kBFloat16 && gate->dim() == 2 && gate->stride(1) == 1 &&
+                    gate->size(0) == T && gate_head_stride >= 0 && gate->size(1) >= (Hq - 1) * gate_head_stride + D,
+                "gate bf16 [T, (Hq - 1) * gate_head_stride + D]");
+    kv8_check_on(kc, *gate, "gate");
+    a.gate = reinterpret_cast<const __nv_bfloat16*>(gate->data_ptr());
+    a.ldg_t = gate->stride(0);
+    a.ldg_h = gate_head_stride;
+  }
+  if (T == 0) return;
+  const c10::cuda::CUDAGuard guard(kc.device());
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
+  a.o = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  a.ldq = q.stride(0);
+  a.ldo = out.stride(0);
+  a.slot = (int)slot; a.T = (int)T; a.p0 = (int)p0; a.Hq = (int)Hq;
+  a.sl2 = (float)scale * 1.4426950408889634f;
+  HX_KV8_LAUNCH(attn_prefill_kv8_launch(a, at::cuda::getCurrentCUDAStream()));
+}
