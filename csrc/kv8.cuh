@@ -32,14 +32,27 @@ constexpr float kKV8Least = 1e-30f;                 // a block below this holds 
 template <bool FP8>
 HX_DEVICE float kv8_top() { return FP8 ? 448.f : 127.f; }
 
+// The codes of four values, the first one in the low byte.
 template <bool FP8>
-HX_DEVICE uint8_t kv8_code(float x, float inv) {
-  const float y = x * inv;
+HX_DEVICE uint32_t kv8_code4(const float* x, float inv) {
   if constexpr (FP8) {
-    return y != y ? (uint8_t)0 : (uint8_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[i] = x[i] * inv;
+      if (y[i] != y[i]) y[i] = 0.f;
+    }
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
   } else {
-    const int c = y != y ? 0 : __float2int_rn(fminf(fmaxf(y, -127.f), 127.f));
-    return (uint8_t)(int8_t)c;
+    int c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // to the nearest, NaN to 0, -inf to -127
+      asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(c[i]) : "f"(x[i] * inv));
+      c[i] = max(c[i], -127);
+    }
+    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
   }
 }
 

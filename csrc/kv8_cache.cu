@@ -74,14 +74,17 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(KV8AppendArgs a) {
     for (int i = 0; i < NP; ++i) {
       if (!isv) {
         const int key = (tid >> 5) * 8 + ((tid & 31) >> 2);
-        alignas(16) uint8_t q[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) q[e] = kv8_code<FP8>(f[i][e], inv);
-        *reinterpret_cast<uint4*>(dst + (i * kKV8Block + key) * 64 + (tid & 3) * 16) = *reinterpret_cast<uint4*>(q);
+        *reinterpret_cast<uint4*>(dst + (i * kKV8Block + key) * 64 + (tid & 3) * 16) =
+            make_uint4(kv8_code4<FP8>(f[i], inv), kv8_code4<FP8>(f[i] + 4, inv), kv8_code4<FP8>(f[i] + 8, inv),
+                       kv8_code4<FP8>(f[i] + 12, inv));
       } else {
         const int d0 = (i * 4 + (tid >> 5)) * 16;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) vcode[(d0 + e) * kKV8Block + (tid & 31)] = kv8_code<FP8>(f[i][e], inv);
+        for (int e = 0; e < 16; e += 4) {
+          const uint32_t q = kv8_code4<FP8>(f[i] + e, inv);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) vcode[(d0 + e + c) * kKV8Block + (tid & 31)] = (uint8_t)(q >> 8 * c);
+        }
       }
     }
     __syncthreads();
