@@ -23,6 +23,8 @@
 // are bf16 ones on q and p split into two bf16 parts (16 bits).
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "kv8.cuh"
 #include "mma_frag.cuh"
 #include "tc_common.cuh"
@@ -32,12 +34,13 @@ namespace cg = cooperative_groups;
 namespace hx {
 
 constexpr int kKV8Warps = 4;   // warps of a CTA
+constexpr int kKV8MaxDevices = 64;
 
 template <int D>
 struct KV8Ring {
   static constexpr int kUnit = (D >= 128 ? 128 : D) * kKV8Block;  // bytes of a copy
   static constexpr int kUK = D * kKV8Block / kUnit;               // copies of a K (or V) block
-  static constexpr int kSlots = D >= 128 ? 6 : 8;                 // slots of a warp's ring
+  static constexpr int kSlots = D >= 128 ? 5 : 8;                 // slots of a warp's ring
 };
 
 template <int D, int NT>
@@ -46,19 +49,22 @@ struct DecodeKV8Smem {
   static constexpr int LD = D + 4;       // row stride of wo: lanes of one store hit distinct banks
   union {
     alignas(128) uint8_t ring[kKV8Warps][KV8Ring<D>::kSlots][KV8Ring<D>::kUnit];
-    float wo[kKV8Warps][GP][LD];         // the warps' O, then (in [0]) the CTA's
+    alignas(16) float wo[kKV8Warps][GP][LD];  // the warps' O, then (in [0]) the CTA's
+    float fw[GP][kKV8MaxPart];           // the partials' weights in the last merge
   };
-  float q[GP][D];                        // normed, rotated, times a power of two
-  float kn[D];                           // the new token's key
+  alignas(16) float q[GP][D];            // normed, rotated, times a power of two
+  alignas(16) uint2 qf[NT][D / 16][32];  // the same as f16 operands, a lane's four values together
+  alignas(16) __nv_bfloat16 knew[D], vnew[D];  // the new token as the cache holds it
+  float ps[kKV8Warps][2 * NT][32][4];    // the warps' parts of the last block's scores
   float cs[D / 2], sn[D / 2];            // rotation of the sequence's position
-  alignas(16) __nv_bfloat16 knew[D], vnew[D];        // the new token as the cache holds it
   float qmul[GP];                        // score factor of each head: scale * log2(e) / power of two
   float wm[kKV8Warps][GP], wl[kKV8Warps][GP];
   float cm[GP], cl[GP];                  // this CTA's (max, sum)
-  float pw[GP][kKV8CL];                  // the cluster's CTAs' weights
-  float fw[GP][kKV8MaxPart];             // the partials' weights in the last merge
+  float lsum[GP];                        // the pair's sums in the last merge
   uint64_t full[kKV8Warps][KV8Ring<D>::kSlots];
   int off[kKV8MaxBatch + 1];             // blocks before sequence b
+  int slot[kKV8MaxBatch], pos[kKV8MaxBatch];
+  int nbmax;
   float red[2][kKV8Warps];
   int last;
 };
@@ -166,25 +172,28 @@ struct DecodeKV8Warp {
 
   // O^T += V^T . P over the 64 dims of panel u (64 dims x 32 codes in shared memory)
   HX_DEVICE void pv_panel(const uint8_t* p, int u, float vs) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pv_tile(p, i, u * 4 + i, vs);
+  }
+
+  // dims 16 i .. 16 i + 15 of a panel, output tile `to`
+  HX_DEVICE void pv_tile(const uint8_t* p, int i, int to, float vs) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint2 x = *reinterpret_cast<const uint2*>(p + (i * 16 + g) * 32 + t * 8);
+    const uint2 y = *reinterpret_cast<const uint2*>(p + (i * 16 + g + 8) * 32 + t * 8);
+    uint32_t a[2][4];
+    codes_to_f16<FP8>(x.x, a[0][0], a[0][2]);
+    codes_to_f16<FP8>(y.x, a[0][1], a[0][3]);
+    codes_to_f16<FP8>(x.y, a[1][0], a[1][2]);
+    codes_to_f16<FP8>(y.y, a[1][1], a[1][3]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint2 x = *reinterpret_cast<const uint2*>(p + (i * 16 + g) * 32 + t * 8);
-      const uint2 y = *reinterpret_cast<const uint2*>(p + (i * 16 + g + 8) * 32 + t * 8);
-      uint32_t a[2][4];
-      codes_to_f16<FP8>(x.x, a[0][0], a[0][2]);
-      codes_to_f16<FP8>(y.x, a[0][1], a[0][3]);
-      codes_to_f16<FP8>(x.y, a[1][0], a[1][2]);
-      codes_to_f16<FP8>(y.y, a[1][1], a[1][3]);
+    for (int nt = 0; nt < NT; ++nt) {
+      float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < 2; ++s) mma_f16(o, a[s][0], a[s][1], a[s][2], a[s][3], pb[s][nt][0], pb[s][nt][1]);
+      float (&c)[4] = acc[to][nt];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) mma_f16(o, a[s][0], a[s][1], a[s][2], a[s][3], pb[s][nt][0], pb[s][nt][1]);
-        float (&c)[4] = acc[u * 4 + i][nt];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = fmaf(c[e], corr[nt][e & 1], o[e] * vs);
-      }
+      for (int e = 0; e < 4; ++e) c[e] = fmaf(c[e], corr[nt][e & 1], o[e] * vs);
     }
   }
 
@@ -244,6 +253,10 @@ HX_DEVICE void split_bf16x2(float x, float y, uint32_t& hi, uint32_t& lo) {
   lo = pack_bf16x2(x - f.x, y - f.y);
 }
 
+HX_DEVICE void add4(float4& o, const float4& v, float f) {
+  o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+}
+
 template <int D, int NT, bool FP8>
 __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(AttnDecodeKV8Args a) {
   using R = KV8Ring<D>;
@@ -266,14 +279,17 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
   pdl_launch_dependents();
   // ---- blocks of each sequence (0: refused), and the blocks before it -------------------------
   if (warp == 0) {
-    int base = 0;
+    int base = 0, most = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       int n = 0;
       if (b0 + lane < a.B) {
         const int slot = a.slots[b0 + lane];
         const int p = slot >= 0 && slot < a.c.S ? a.pos[slot] : -1;
         n = p >= 0 && p < a.c.nb * kKV8Block ? p / kKV8Block + 1 : 0;
+        s->slot[b0 + lane] = slot;
+        s->pos[b0 + lane] = p;
       }
+      most = max(most, n);
       int x = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -283,7 +299,12 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       if (b0 + lane < a.B) s->off[b0 + lane + 1] = base + x;
       base += __shfl_sync(0xffffffffu, x, 31);
     }
-    if (lane == 0) s->off[0] = 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) {
+      s->off[0] = 0;
+      s->nbmax = most;
+    }
   }
   __syncthreads();
   if (cid == 0 && crank == 0)  // refused sequences: no cache access, a zero row, the error word
@@ -294,35 +315,40 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       }
   // Runs of `chunk` blocks. At least a block for every warp of the cluster where a pair has as
   // many: a pair split further would only add partials to merge.
-  const long long W = (long long)s->off[a.B] * PB;
-  int nbmax = 0;
-  for (int b = 0; b < a.B; ++b) nbmax = max(nbmax, s->off[b + 1] - s->off[b]);
-  const long long chunk = max((W + NC - 1) / NC, (long long)min(nbmax, CL * NW));
-  long long w = cid * chunk;
-  const long long wend = min(W, w + chunk);
-  if (w >= wend) return;  // the whole cluster
+  const int W = s->off[a.B] * PB;  // the host has checked that it fits
+  const int chunk = max((W + NC - 1) / NC, min(s->nbmax, CL * NW));
+  if ((long long)cid * chunk >= W) return;  // the whole cluster
+  int w = cid * chunk;
+  const int wend = min(W - w, chunk) + w;
   float* part_o = reinterpret_cast<float*>(a.ws + kKV8PartAt);  // [NC + pairs][GP][D]
-  float* part_ml = part_o + (long long)(NC + a.B * PB) * GP * D;  // [NC + pairs][GP][2]
+  float2* part_ml = reinterpret_cast<float2*>(part_o + (long long)(NC + a.B * PB) * GP * D);  // [NC + pairs][GP]
   unsigned seq = 0;  // copies this warp has issued in all
   bool ok = true;
   DecodeKV8Warp<D, NT, FP8> st;
   int b = 0;
+  for (int lo = 0, hi = a.B; lo < hi;) {  // the sequence of the run's first block
+    b = (lo + hi) / 2;
+    if (s->off[b + 1] * PB <= w) lo = b + 1;
+    else hi = b;
+    b = lo;
+  }
   while (w < wend) {
-    while ((long long)s->off[b + 1] * PB <= w) ++b;
+    while (s->off[b + 1] * PB <= w) ++b;
     const int nb = s->off[b + 1] - s->off[b];
-    const int pl = (int)((w - (long long)s->off[b] * PB) / nb);      // kv head and head group
-    const long long p0 = (long long)s->off[b] * PB + (long long)pl * nb;  // the pair's first block in the list
-    const int blk0 = (int)(w - p0), blk1 = (int)min((long long)nb, wend - p0);
+    const int pl = (w - s->off[b] * PB) / nb;  // kv head and head group
+    const int p0 = s->off[b] * PB + pl * nb;   // the pair's first block in the list
+    const int blk0 = w - p0, blk1 = min(nb, wend - p0);
     const int pair = b * PB + pl, h = pl / HG, hg = pl % HG, g0 = hg * per, n = min(per, G - g0);
-    const int slot = a.slots[b], p = a.pos[slot], row = p % kKV8Block;
+    const int slot = s->slot[b], p = s->pos[b], row = p % kKV8Block;
     const __nv_bfloat16* pr = a.proj + b * a.ldp;
     // ---- this warp's blocks: blk0 + gw, + CL * NW, ...; the sequence's last block is not copied --
     const int gw = crank * NW + warp;
     const int my0 = blk0 + gw;
     const int n8 = min(blk1, nb - 1);
     const int mine = my0 < n8 ? (n8 - my0 + CL * NW - 1) / (CL * NW) : 0;  // complete blocks
-    const bool has_last = blk1 == nb && (nb - 1 - blk0) % (CL * NW) == gw;
     const bool cta_last = blk1 == nb && (nb - 1 - blk0) % (CL * NW) / NW == crank;
+    const bool completes = cta_last && row == kKV8Block - 1;
+    const int host = (nb - 1 - blk0) % NW;  // the warp whose ring holds the codes of a completed block
     const unsigned units = (unsigned)mine * 2 * R::kUK;
     const uint8_t* kbase = a.c.kc + a.c.block(slot, h, 0) * (D * kKV8Block);
     const uint8_t* vbase = a.c.vc + a.c.block(slot, h, 0) * (D * kKV8Block);
@@ -333,190 +359,272 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       tc::mbar_expect_tx(&s->full[warp][sl], R::kUnit);
       bulk_load(s->ring[warp][sl], src, R::kUnit, &s->full[warp][sl]);
     };
-    // (the warp with the last block starts its copies after it: the block's codes may be made in
-    // its ring)
-    if (lane == 0 && ok && !has_last)
-      for (unsigned i = 0; i < min(units, (unsigned)R::kSlots); ++i) issue(i);
-    // ---- q of the group's heads (and the new key): norm, rotation ------------------------------
+    auto fill = [&] {
+      if (lane == 0 && ok)
+        for (unsigned i = 0; i < min(units, (unsigned)R::kSlots); ++i) issue(i);
+    };
+    if (!(completes && warp == host)) fill();
+    // ---- loads of all that the segment's start needs, in flight together -------------------------
+    const int nrow = n + (cta_last ? 1 : 0);  // the group's queries, then the new key
+    constexpr int NR = (GP + NW) / NW;
+    __nv_bfloat16 xr[NR][D / 32], xv[D / 32];
+    float wq[D / 32], wk[D / 32];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int r = warp + i * NW;
+      const __nv_bfloat16* src = r == n ? pr + a.Hq * qw + h * D : pr + (long long)(h * G + g0 + r) * qw;
+      if (r < nrow)
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) xr[i][e] = src[e * 32 + lane];
+    }
+    const bool kwarp = cta_last && warp == n % NW;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      wq[e] = a.q_norm_w ? a.q_norm_w[e * 32 + lane] : 1.f;
+      wk[e] = kwarp && a.k_norm_w ? a.k_norm_w[e * 32 + lane] : 1.f;
+      if (kwarp) xv[e] = pr[a.Hq * qw + (Hkv + h) * D + e * 32 + lane];
+    }
+    // The last block's bf16 rows, for the whole CTA: for a completed block 16-value pieces of the
+    // block's layout (X[i][0..1] of K, [2..3] of V); else operands: warp w takes dims groups
+    // (of 16) w * NP + i of the sums and of the output.
+    uint4 X[NP][4];
+    __nv_bfloat16* kt = a.c.kt + a.c.head(slot, h) * (NP * kKV8Panel);
+    __nv_bfloat16* vt = a.c.vt + a.c.head(slot, h) * (NP * kKV8Panel);
+    if (cta_last) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (completes) {
+          const int c = i * NTH + tid;
+          X[i][0] = *reinterpret_cast<const uint4*>(kt + c * 16);
+          X[i][1] = *reinterpret_cast<const uint4*>(kt + c * 16 + 8);
+          X[i][2] = *reinterpret_cast<const uint4*>(vt + c * 16);
+          X[i][3] = *reinterpret_cast<const uint4*>(vt + c * 16 + 8);
+        } else {
+          const int k = warp * NP + i;
+#pragma unroll
+          for (int sx = 0; sx < 2; ++sx) {
+            const __nv_bfloat16* src = kt + (k >> 2) * kKV8Panel + t * 16 + (k & 3) * 4;
+            const uint2 u0 = *reinterpret_cast<const uint2*>(src + key_of(sx, 0, g) * 64);
+            const uint2 u1 = *reinterpret_cast<const uint2*>(src + key_of(sx, 1, g) * 64);
+            X[i][sx] = make_uint4(u0.x, u0.y, u1.x, u1.y);
+            X[i][2 + sx] = *reinterpret_cast<const uint4*>(vt + (k * 16 + g + 8 * sx) * kKV8Block + t * 8);
+          }
+        }
+      }
+    }
     const int prot = p + (a.rope_delta ? a.rope_delta[slot] : 0);
     for (int i = tid; i < a.rot / 2; i += NTH) sincosf((float)prot * a.inv_freq[i], &s->sn[i], &s->cs[i]);
     __syncthreads();
-    for (int r = warp; r < n + (cta_last ? 1 : 0); r += NW) {
+    // ---- q of the group's heads (and the new key): norm, rotation ------------------------------
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int r = warp + i * NW;
+      if (r >= nrow) break;
       const bool isk = r == n;
-      const __nv_bfloat16* src = isk ? pr + a.Hq * qw + h * D : pr + (long long)(h * G + g0 + r) * qw;
-      const float* nw = isk ? a.k_norm_w : a.q_norm_w;
-      float* x = isk ? s->kn : s->q[r];
       float v[D / 32];
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        v[i] = __bfloat162float(src[i * 32 + lane]);
-        ss += v[i] * v[i];
+      for (int e = 0; e < D / 32; ++e) {
+        v[e] = __bfloat162float(xr[i][e]);
+        ss += v[e] * v[e];
       }
-      if (nw) {
+      if (isk ? a.k_norm_w : a.q_norm_w) {
         const float inv = rsqrtf(warp_sum(ss) / D + a.eps);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) v[i] *= inv * nw[i * 32 + lane];
+        for (int e = 0; e < D / 32; ++e) v[e] *= inv * (isk ? wk[e] : wq[e]);
       }
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) x[i * 32 + lane] = v[i];
-      __syncwarp();
       const int half = a.rot / 2;
+      if (half) {
+        float* x = isk ? s->ps[warp][0][0] : s->q[r];  // D floats that only this warp uses
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const int d = i * 32 + lane;
-        if (d < a.rot) v[i] = d < half ? v[i] * s->cs[d] - x[d + half] * s->sn[d]
-                                       : v[i] * s->cs[d - half] + x[d - half] * s->sn[d - half];
+        for (int e = 0; e < D / 32; ++e) x[e * 32 + lane] = v[e];
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const int d = e * 32 + lane;
+          if (d < a.rot) v[e] = d < half ? v[e] * s->cs[d] - x[d + half] * s->sn[d]
+                                         : v[e] * s->cs[d - half] + x[d - half] * s->sn[d - half];
+        }
+        __syncwarp();
       }
-      __syncwarp();
       if (isk) {
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const int d = i * 32 + lane;
-          s->knew[d] = __float2bfloat16(v[i]);
-          s->vnew[d] = pr[a.Hq * qw + (Hkv + h) * D + d];
+        for (int e = 0; e < D / 32; ++e) {
+          s->knew[e * 32 + lane] = __float2bfloat16(v[e]);
+          s->vnew[e * 32 + lane] = xv[e];
         }
       } else {
         float mag = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) mag = fmaxf(mag, kv8_mag(v[i]));
+        for (int e = 0; e < D / 32; ++e) mag = fmaxf(mag, kv8_mag(v[e]));
         mag = warp_max(mag);
         // power of two that brings the largest entry to 128..256
         const int ex = min(134 - (int)(__float_as_uint(mag) >> 23), 120);
         const float up = __uint_as_float((uint32_t)(ex + 127) << 23);
+        __half* qf = reinterpret_cast<__half*>(s->qf[r >> 3]);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) x[i * 32 + lane] = v[i] * up;
+        for (int e = 0; e < D / 32; ++e) {
+          const int d = e * 32 + lane;
+          if (cta_last) s->q[r][d] = v[e] * up;
+          // lane 4 (r % 8) + (d / 16) % 4 of dims group 4 (d / 64) + (d / 4) % 4 holds d % 4
+          const int k = (d >> 6) * 4 + ((d >> 2) & 3), l = (r & 7) * 4 + ((d >> 4) & 3);
+          qf[(k * 32 + l) * 4 + (d & 3)] = __float2half_rn(v[e] * up);
+        }
         if (lane == 0) s->qmul[r] = a.sl2 / up;
       }
     }
     __syncthreads();
-    if (cta_last && hg == 0) {  // the new token enters the tail
-      __nv_bfloat16* kt = a.c.kt + a.c.head(slot, h) * (NP * kKV8Panel);
-      __nv_bfloat16* vt = a.c.vt + a.c.head(slot, h) * (NP * kKV8Panel);
-      for (int d = tid; d < D; d += NTH) {
-        kt[((d >> 6) * kKV8Block + row) * 64 + (d & 63)] = s->knew[d];
-        vt[d * kKV8Block + row] = s->vnew[d];
+    st.reset();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const bool in = nt * 8 + g < n;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const uint2 x = s->qf[nt][k][lane];
+        st.qb[nt][k][0] = in ? x.x : 0u;
+        st.qb[nt][k][1] = in ? x.y : 0u;
       }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) st.mul[nt][e] = nt * 8 + 2 * t + e < n ? s->qmul[nt * 8 + 2 * t + e] : 0.f;
     }
-    // A block that this token completes gets its codes: into the ring of the warp that attends to
-    // it and into the cache. Every head group derives them; the first one stores them.
-    const bool completes = cta_last && row == kKV8Block - 1;
-    uint8_t* fresh = s->ring[(nb - 1 - blk0) % NW][0];  // that warp's ring, not in use yet
-    float scale[2];
-    if (completes) {
-      uint4 x[2][NP][2];
-      float mag[2] = {0.f, 0.f};
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        const __nv_bfloat16* src = (z ? a.c.vt : a.c.kt) + a.c.head(slot, h) * (NP * kKV8Panel);
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {  // 16 values from c * 16 on of the block's layout
-          const int c = i * NTH + tid;
-          x[z][i][0] = *reinterpret_cast<const uint4*>(src + c * 16);
-          x[z][i][1] = *reinterpret_cast<const uint4*>(src + c * 16 + 8);
-          if (z) {
-            if (c & 1)  // key 31 of dim c / 2
-              x[z][i][1].w = (x[z][i][1].w & 0xffffu) | (uint32_t)__bfloat16_as_ushort(s->vnew[c >> 1]) << 16;
-          } else if ((c & 127) >= 124) {  // key 31 of panel c / 128
-            const uint4* kn = reinterpret_cast<const uint4*>(s->knew + (c >> 7) * 64 + (c & 3) * 16);
-            x[z][i][0] = kn[0];
-            x[z][i][1] = kn[1];
-          }
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float f[8];
-            unpack8(*reinterpret_cast<const bf16x8*>(&x[z][i][q]), f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mag[z] = fmaxf(mag[z], kv8_mag(f[e]));
-          }
+    // ---- the sequence's last block, by the whole CTA ------------------------------------------------
+    if (cta_last) {
+      if (hg == 0)  // the new token enters the tail
+        for (int d = tid; d < D; d += NTH) {
+          kt[((d >> 6) * kKV8Block + row) * 64 + (d & 63)] = s->knew[d];
+          vt[d * kKV8Block + row] = s->vnew[d];
         }
-        mag[z] = warp_max(mag[z]);
-        if (lane == 0) s->red[z][warp] = mag[z];
-      }
-      __syncthreads();
-      const long long at = a.c.block(slot, h, nb - 1);
-#pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        const float m = fmaxf(fmaxf(s->red[z][0], s->red[z][1]), fmaxf(s->red[z][2], s->red[z][3]));
-        const float inv = kv8_inv<FP8>(m);
-        scale[z] = kv8_scale<FP8>(m);
-        uint8_t* dst = (z ? a.c.vc : a.c.kc) + at * (D * kKV8Block);
+      float ksc = 1.f, vsc = 1.f;
+      uint8_t* fresh = s->ring[host][0];
+      st.clear_scores();
+      if (completes) {
+        // Its codes, into the ring (that warp has no copies under way) and into the cache. Every
+        // head group derives them; the first one stores them.
+        float mag[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-          float f[16];
-          unpack8(*reinterpret_cast<const bf16x8*>(&x[z][i][0]), f);
-          unpack8(*reinterpret_cast<const bf16x8*>(&x[z][i][1]), f + 8);
-          const uint4 v = make_uint4(kv8_code4<FP8>(f, inv), kv8_code4<FP8>(f + 4, inv), kv8_code4<FP8>(f + 8, inv),
-                                     kv8_code4<FP8>(f + 12, inv));
-          reinterpret_cast<uint4*>(fresh + z * D * kKV8Block)[i * NTH + tid] = v;
-          if (hg == 0) reinterpret_cast<uint4*>(dst)[i * NTH + tid] = v;
-        }
-        if (hg == 0 && tid == 0) (z ? a.c.vs : a.c.ks)[at] = scale[z];
-      }
-      __syncthreads();
-    }
-    st.reset();
-    if (mine > 0 || has_last) {
+          const int c = i * NTH + tid;
+          if ((c & 127) >= 124) {  // key 31 of K's panel c / 128
+            const uint4* kn = reinterpret_cast<const uint4*>(s->knew + (c >> 7) * 64 + (c & 3) * 16);
+            X[i][0] = kn[0];
+            X[i][1] = kn[1];
+          }
+          if (c & 1)  // key 31 of V's dim c / 2
+            X[i][3].w = (X[i][3].w & 0xffffu) | (uint32_t)__bfloat16_as_ushort(s->vnew[c >> 1]) << 16;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const bool in = nt * 8 + g < n;
-        const float* q = s->q[nt * 8 + g];
+          for (int q = 0; q < 4; ++q) {
+            float f[8];
+            unpack8(*reinterpret_cast<const bf16x8*>(&X[i][q]), f);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const int d = (k >> 2) * 64 + t * 16 + (k & 3) * 4;
-          const float4 x = *reinterpret_cast<const float4*>(q + d);
-          st.qb[nt][k][0] = in ? pack_f16x2(x.x, x.y) : 0u;
-          st.qb[nt][k][1] = in ? pack_f16x2(x.z, x.w) : 0u;
+            for (int e = 0; e < 8; ++e) mag[q >> 1] = fmaxf(mag[q >> 1], kv8_mag(f[e]));
+          }
         }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) st.mul[nt][e] = nt * 8 + 2 * t + e < n ? s->qmul[nt * 8 + 2 * t + e] : 0.f;
-      }
-    }
-    // ---- the sequence's last block: bf16 rows of the tail and the new token ----------------------
-    if (has_last) {
-      const __nv_bfloat16* kt = a.c.kt + a.c.head(slot, h) * (NP * kKV8Panel);
-      const __nv_bfloat16* vt = a.c.vt + a.c.head(slot, h) * (NP * kKV8Panel);
-      if (completes) {
-        st.clear_scores();
+        for (int z = 0; z < 2; ++z) {
+          mag[z] = warp_max(mag[z]);
+          if (lane == 0) s->red[z][warp] = mag[z];
+        }
+        __syncthreads();
+        const long long at = a.c.block(slot, h, nb - 1);
 #pragma unroll
-        for (int q = 0; q < NP; ++q) st.qk_panel(fresh + q * kKV8Panel, q);
-        st.softmax(scale[0], kKV8Block);
-        st.pack_p();
+        for (int z = 0; z < 2; ++z) {
+          const float m = fmaxf(fmaxf(s->red[z][0], s->red[z][1]), fmaxf(s->red[z][2], s->red[z][3]));
+          const float inv = kv8_inv<FP8>(m);
+          (z ? vsc : ksc) = kv8_scale<FP8>(m);
+          uint8_t* dst = (z ? a.c.vc : a.c.kc) + at * (D * kKV8Block);
 #pragma unroll
-        for (int q = 0; q < NP; ++q) st.pv_panel(fresh + D * kKV8Block + q * kKV8Panel, q, scale[1]);
-      } else {
-        st.clear_scores();
-#pragma unroll 1
-        for (int pn = 0; pn < NP; ++pn)
+          for (int i = 0; i < NP; ++i) {
+            float f[16];
+            unpack8(*reinterpret_cast<const bf16x8*>(&X[i][2 * z]), f);
+            unpack8(*reinterpret_cast<const bf16x8*>(&X[i][2 * z + 1]), f + 8);
+            const uint4 v = make_uint4(kv8_code4<FP8>(f, inv), kv8_code4<FP8>(f + 4, inv),
+                                       kv8_code4<FP8>(f + 8, inv), kv8_code4<FP8>(f + 12, inv));
+            reinterpret_cast<uint4*>(fresh + z * D * kKV8Block)[i * NTH + tid] = v;
+            if (hg == 0) reinterpret_cast<uint4*>(dst)[i * NTH + tid] = v;
+          }
+          if (hg == 0 && tid == 0) (z ? a.c.vs : a.c.ks)[at] = z ? vsc : ksc;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int k = warp * NP + i;
+          const uint8_t* src = fresh + (k >> 2) * kKV8Panel + t * 16 + (k & 3) * 4;
 #pragma unroll
           for (int sx = 0; sx < 2; ++sx) {
-            uint32_t kx[2][8];
+            uint32_t a0, a1, a2, a3;
+            codes_to_f16<FP8>(*reinterpret_cast<const uint32_t*>(src + key_of(sx, 0, g) * 64), a0, a2);
+            codes_to_f16<FP8>(*reinterpret_cast<const uint32_t*>(src + key_of(sx, 1, g) * 64), a1, a3);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              // rows past the new token hold anything: their scores are replaced in softmax()
-              const int key = key_of(sx, j, g);
-              const __nv_bfloat16* r = key == row ? s->knew + pn * 64 : kt + (pn * kKV8Block + key) * 64;
-              const uint4 x = *reinterpret_cast<const uint4*>(r + t * 16);
-              const uint4 y = *reinterpret_cast<const uint4*>(r + t * 16 + 8);
-              kx[j][0] = x.x; kx[j][1] = x.y; kx[j][2] = x.z; kx[j][3] = x.w;
-              kx[j][4] = y.x; kx[j][5] = y.y; kx[j][6] = y.z; kx[j][7] = y.w;
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint2 x = s->qf[nt][k][lane];
+              const bool in = nt * 8 + g < n;
+              mma_f16(st.sc[sx][nt], a0, a1, a2, a3, in ? x.x : 0u, in ? x.y : 0u);
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                const int hr = nt * 8 + g;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (hr < n) x = *reinterpret_cast<const float4*>(s->q[hr] + pn * 64 + t * 16 + k * 4);
-                uint32_t h0, l0, h1, l1;
-                split_bf16x2(x.x, x.y, h0, l0);
-                split_bf16x2(x.z, x.w, h1, l1);
-                mma_16816(st.sc[sx][nt], kx[0][2 * k], kx[1][2 * k], kx[0][2 * k + 1], kx[1][2 * k + 1], h0, h1);
-                mma_16816(st.sc[sx][nt], kx[0][2 * k], kx[1][2 * k], kx[0][2 * k + 1], kx[1][2 * k + 1], l0, l1);
-              }
           }
-        st.softmax(1.f, row);
-        uint32_t ph[2][NT][2], plo[2][NT][2];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const int k = warp * NP + i, d = (k >> 2) * 64 + t * 16 + (k & 3) * 4;
+          const uint2 kn = *reinterpret_cast<const uint2*>(s->knew + d);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int hr = nt * 8 + g;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (hr < n) x = *reinterpret_cast<const float4*>(s->q[hr] + d);
+            uint32_t h0, l0, h1, l1;
+            split_bf16x2(x.x, x.y, h0, l0);
+            split_bf16x2(x.z, x.w, h1, l1);
+#pragma unroll
+            for (int sx = 0; sx < 2; ++sx) {
+              // rows past the new token hold anything: their scores are replaced in softmax()
+              uint4 y = X[i][sx];
+              if (key_of(sx, 0, g) == row) { y.x = kn.x; y.y = kn.y; }
+              if (key_of(sx, 1, g) == row) { y.z = kn.x; y.w = kn.y; }
+              mma_16816(st.sc[sx][nt], y.x, y.z, y.y, y.w, h0, h1);
+              mma_16816(st.sc[sx][nt], y.x, y.z, y.y, y.w, l0, l1);
+            }
+          }
+        }
+      }
+      // The warps' parts of the scores add up to the same probabilities in every warp. Warp 0
+      // alone counts their sum; each adds its own dims of the output.
+#pragma unroll
+      for (int sx = 0; sx < 2; ++sx)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          *reinterpret_cast<float4*>(s->ps[warp][sx * NT + nt][lane]) =
+              make_float4(st.sc[sx][nt][0], st.sc[sx][nt][1], st.sc[sx][nt][2], st.sc[sx][nt][3]);
+      __syncthreads();
+#pragma unroll
+      for (int sx = 0; sx < 2; ++sx)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int y = 0; y < NW; ++y) {
+            const float4 z = *reinterpret_cast<const float4*>(s->ps[y][sx * NT + nt][lane]);
+            x.x += z.x; x.y += z.y; x.z += z.z; x.w += z.w;
+          }
+          st.sc[sx][nt][0] = x.x; st.sc[sx][nt][1] = x.y; st.sc[sx][nt][2] = x.z; st.sc[sx][nt][3] = x.w;
+        }
+      st.softmax(ksc, row);
+      if (warp != 0)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) st.l[nt][0] = st.l[nt][1] = 0.f;
+      if (completes) {
+        st.pack_p();
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+          const uint8_t* src = fresh + D * kKV8Block + q * kKV8Panel;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if ((q * 4 + i) / NP != warp) continue;
+            st.pv_tile(src, i, q * 4 + i, vsc);
+          }
+        }
+      } else {
+        uint32_t ph[2][NT][2], pl2[2][NT][2];
 #pragma unroll
         for (int sx = 0; sx < 2; ++sx)
 #pragma unroll
@@ -526,12 +634,11 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
               uint32_t hi, lo;
               split_bf16x2(st.sc[sx][nt][2 * j], st.sc[sx][nt][2 * j + 1], hi, lo);
               ph[sx][nt][j] = movmatrix_t(hi);
-              plo[sx][nt][j] = movmatrix_t(lo);
+              pl2[sx][nt][j] = movmatrix_t(lo);
             }
         // keys 8t .. 8t+7 of a dim: the new token's value goes in, keys past it are cleared
         // (a probability of zero does not silence an infinity or a NaN)
-        auto vload = [&](int d, uint32_t (&x)[4]) {
-          const uint4 v = *reinterpret_cast<const uint4*>(vt + d * kKV8Block + t * 8);
+        auto clean = [&](int d, uint4 v, uint32_t (&x)[4]) {
           x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
           const uint32_t nv = __bfloat16_as_ushort(s->vnew[d]);
 #pragma unroll
@@ -544,27 +651,29 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         };
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
+          if (i / NP != warp) continue;
           uint32_t x[4], y[4];
-          vload(i * 16 + g, x);
-          vload(i * 16 + g + 8, y);
+          clean(i * 16 + g, X[i % NP][2], x);
+          clean(i * 16 + g + 8, X[i % NP][3], y);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float o[4] = {0.f, 0.f, 0.f, 0.f};
+            float (&o)[4] = st.acc[i][nt];  // still zero: this block is the first
 #pragma unroll
             for (int sx = 0; sx < 2; ++sx) {
               mma_16816(o, x[2 * sx], y[2 * sx], x[2 * sx + 1], y[2 * sx + 1], ph[sx][nt][0], ph[sx][nt][1]);
-              mma_16816(o, x[2 * sx], y[2 * sx], x[2 * sx + 1], y[2 * sx + 1], plo[sx][nt][0], plo[sx][nt][1]);
+              mma_16816(o, x[2 * sx], y[2 * sx], x[2 * sx + 1], y[2 * sx + 1], pl2[sx][nt][0], pl2[sx][nt][1]);
             }
-            float (&c)[4] = st.acc[i][nt];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[e] = fmaf(c[e], st.corr[nt][e & 1], o[e]);
           }
         }
       }
-      if (completes) tc::fence_proxy_async_smem();  // codes in the ring before copies into it
-      __syncwarp();
-      if (lane == 0 && ok)
-        for (unsigned i = 0; i < min(units, (unsigned)R::kSlots); ++i) issue(i);
+      if (completes) {
+        __syncthreads();  // every warp is done with the codes
+        if (warp == host) {
+          tc::fence_proxy_async_smem();  // their stores before the copies into the same memory
+          __syncwarp();
+          fill();
+        }
+      }
     }
     // ---- complete blocks -----------------------------------------------------------------------
     const float* ksp = a.c.ks + a.c.block(slot, h, 0);
@@ -621,103 +730,116 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
 #pragma unroll
         for (int c = 0; c < 4; ++c) s->wo[warp][nt * 8 + 2 * t + (c & 1)][i * 16 + g + (c >> 1) * 8] = st.acc[i][nt][c];
     __syncthreads();
-    for (int i = tid; i < n * D; i += NTH) {
-      const int r = i / D, d = i % D;
-      float M = -INFINITY;
+    for (int i = tid; i < n * (D / 4); i += NTH) {  // four dims of one head
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float M = -INFINITY, L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int x = 0; x < NW; ++x) M = fmaxf(M, s->wm[x][r]);
-      float O = 0.f, L = 0.f;
-      if (M != -INFINITY)
 #pragma unroll
-        for (int x = 0; x < NW; ++x) {
-          const float f = exp2f(s->wm[x][r] - M);
-          O = fmaf(s->wo[x][r][d], f, O);
-          L = fmaf(s->wl[x][r], f, L);
-        }
-      s->wo[0][r][d] = O;  // this thread alone reads and writes (r, d)
+      for (int x = 0; x < NW; ++x) {
+        const float f = s->wm[x][r] == -INFINITY ? 0.f : exp2f(s->wm[x][r] - M);
+        add4(O, *reinterpret_cast<const float4*>(&s->wo[x][r][d]), f);
+        L = fmaf(s->wl[x][r], f, L);
+      }
+      *reinterpret_cast<float4*>(&s->wo[0][r][d]) = O;  // this thread alone reads and writes them
       if (d == 0) { s->cm[r] = M; s->cl[r] = L; }
     }
     // ---- merge the cluster's CTAs: each finishes 1 / CL of the columns -------------------
     cluster.sync();
-    if (tid < n) {
-      float m[CL], M = -INFINITY, L = 0.f;
+    auto finish = [&](int r, int d, float4 o, float l) {  // four dims of the output
+      const int hq = h * G + g0 + r;
+      float f[4] = {o.x / l, o.y / l, o.z / l, o.w / l};
+      if (a.gated) {
+        const __nv_bfloat16* gp = pr + (long long)hq * qw + D + d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = f[e] / (1.f + __expf(-__bfloat162float(gp[e])));
+      }
+      uint2 y;
+      y.x = pack_bf16x2(f[0], f[1]);
+      y.y = pack_bf16x2(f[2], f[3]);
+      *reinterpret_cast<uint2*>(a.out + ((long long)b * a.Hq + hq) * D + d) = y;
+    };
+    const bool alone = blk0 == 0 && blk1 == nb;
+    const int cols = n * (D / 4) / CL, c0 = crank * cols;  // in fours
+    for (int i = c0 + tid; i < c0 + cols; i += NTH) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float m[CL], l[CL], M = -INFINITY, L = 0.f;
+      float4 v[CL], O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int x = 0; x < CL; ++x) {
-        m[x] = *cluster.map_shared_rank(&s->cm[tid], x);
-        M = fmaxf(M, m[x]);
+        m[x] = *cluster.map_shared_rank(&s->cm[r], x);
+        l[x] = *cluster.map_shared_rank(&s->cl[r], x);
+        v[x] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&s->wo[0][r][d], x));
       }
+#pragma unroll
+      for (int x = 0; x < CL; ++x) M = fmaxf(M, m[x]);
 #pragma unroll
       for (int x = 0; x < CL; ++x) {
         const float f = m[x] == -INFINITY ? 0.f : exp2f(m[x] - M);
-        L = fmaf(*cluster.map_shared_rank(&s->cl[tid], x), f, L);
-        s->pw[tid][x] = f;
+        L = fmaf(l[x], f, L);
+        add4(O, v[x], f);
       }
-      s->wm[0][tid] = M;
-      s->wl[0][tid] = L;
-    }
-    __syncthreads();
-    auto finish = [&](int r, int d, float o) {  // o: the row's output
-      const int hq = h * G + g0 + r;
-      if (a.gated) o = o / (1.f + __expf(-__bfloat162float(pr[(long long)hq * qw + D + d])));
-      a.out[((long long)b * a.Hq + hq) * D + d] = __float2bfloat16(o);
-    };
-    const bool alone = blk0 == 0 && blk1 == nb;
-    const int cols = n * D / CL;
-    const long long at = (cid + pair) * (long long)(GP * D);
-    for (int i = crank * cols + tid; i < (crank + 1) * cols; i += NTH) {
-      const int r = i / D, d = i % D;
-      float O = 0.f;
-#pragma unroll
-      for (int x = 0; x < CL; ++x) O = fmaf(cluster.map_shared_rank(&s->wo[0][r][0], x)[d], s->pw[r][x], O);
-      if (alone) finish(r, d, O / s->wl[0][r]);
-      else part_o[at + i] = O;
-    }
-    if (!alone) {
-      if (crank == 0 && tid < n) {
-        part_ml[((long long)(cid + pair) * GP + tid) * 2] = s->wm[0][tid];
-        part_ml[((long long)(cid + pair) * GP + tid) * 2 + 1] = s->wl[0][tid];
+      if (alone) {
+        finish(r, d, O, L);
+      } else {
+        reinterpret_cast<float4*>(part_o + (long long)(cid + pair) * (GP * D))[i] = O;
+        if (d == 0) part_ml[(long long)(cid + pair) * GP + r] = make_float2(M, L);
       }
-      __threadfence();
     }
+    if (!alone) __threadfence();
     tc::fence_proxy_async_smem();  // O's stores before the next segment's copies into the same memory
     cluster.sync();
     if (!alone) {
       // the cluster that completes the pair's block count merges its partials
       if (crank == 0 && tid == 0) {
         int* counter = a.ws + kKV8Err + pair;
-        const int done = atomicAdd(counter, blk1 - blk0) + (blk1 - blk0);
-        if (done == nb) *counter = 0;
-        const int last = done == nb;
-        for (int x = 0; x < CL; ++x) *cluster.map_shared_rank(&s->last, x) = last;
+        const int last = atomicAdd(counter, blk1 - blk0) + (blk1 - blk0) == nb;
+        if (last) *counter = 0;
         __threadfence();
+        for (int x = 0; x < CL; ++x) *cluster.map_shared_rank(&s->last, x) = last;
       }
       cluster.sync();
       if (s->last) {
         __threadfence();
-        const int c0 = (int)(p0 / chunk), np = (int)((p0 + nb - 1) / chunk) - c0 + 1;  // its clusters
-        for (int r = warp; r < n; r += NW) {
-          float M = -INFINITY;
-          for (int x = lane; x < np; x += 32) M = fmaxf(M, __ldcg(&part_ml[((long long)(c0 + x + pair) * GP + r) * 2]));
+        const int f0 = p0 / chunk, np = (p0 + nb - 1) / chunk - f0 + 1;  // its clusters
+        const long long q0 = f0 + pair;
+        const int r0 = c0 / (D / 4), r1 = (c0 + cols - 1) / (D / 4);       // heads of this CTA's columns
+        for (int r = r0 + warp; r <= r1; r += NW) {
+          constexpr int NX = (kKV8MaxPart + 31) / 32;
+          float2 ml[NX];
+          float M = -INFINITY, L = 0.f;
+#pragma unroll
+          for (int x = 0; x < NX; ++x)
+            ml[x] = x * 32 + lane < np ? __ldcg(&part_ml[(q0 + x * 32 + lane) * GP + r]) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+          for (int x = 0; x < NX; ++x) M = fmaxf(M, ml[x].x);
           M = warp_max(M);
-          float L = 0.f;
-          for (int x = lane; x < np; x += 32) {
-            const long long j = ((long long)(c0 + x + pair) * GP + r) * 2;
-            const float f = exp2f(__ldcg(&part_ml[j]) - M);
-            L = fmaf(__ldcg(&part_ml[j + 1]), f, L);
-            s->fw[r][x] = f;
+#pragma unroll
+          for (int x = 0; x < NX; ++x) {
+            const float f = ml[x].x == -INFINITY ? 0.f : exp2f(ml[x].x - M);
+            if (x * 32 + lane < np) s->fw[r][x * 32 + lane] = f;
+            L = fmaf(ml[x].y, f, L);
           }
           L = warp_sum(L);
-          if (lane == 0) s->wl[0][r] = L;
+          if (lane == 0) s->lsum[r] = L;
         }
         __syncthreads();
-        for (int i = crank * cols + tid; i < (crank + 1) * cols; i += NTH) {
-          const int r = i / D, d = i % D;
-          float O = 0.f;
-#pragma unroll 8
-          for (int x = 0; x < np; ++x)
-            O = fmaf(__ldcg(&part_o[(long long)(c0 + x + pair) * (GP * D) + i]), s->fw[r][x], O);
-          finish(r, d, O / s->wl[0][r]);
+        for (int i = c0 + tid; i < c0 + cols; i += NTH) {
+          const int r = i / (D / 4), d = i % (D / 4) * 4;
+          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int x = 0; x < np; x += 16) {  // sixteen loads in flight
+            float4 v[16];
+#pragma unroll
+            for (int y = 0; y < 16; ++y)
+              v[y] = x + y < np ? __ldcg(reinterpret_cast<const float4*>(part_o + (q0 + x + y) * (GP * D)) + i)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int y = 0; y < 16; ++y) add4(O, v[y], x + y < np ? s->fw[r][x + y] : 0.f);
+          }
+          finish(r, d, O, s->lsum[r]);
         }
+        tc::fence_proxy_async_smem();  // the weights lie in the ring's memory
         __syncthreads();
       }
     }
@@ -726,12 +848,37 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
 }
 
 template <int D, int NT, bool FP8>
-static cudaError_t launch_decode(const AttnDecodeKV8Args& a, cudaStream_t st) {
+static cudaError_t launch_decode(AttnDecodeKV8Args a, cudaStream_t st) {
   auto k = attn_decode_kv8_kernel<D, NT, FP8>;
   const size_t smem = sizeof(DecodeKV8Smem<D, NT>);
   static_assert(sizeof(DecodeKV8Smem<D, NT>) <= 113 * 1024, "two CTAs of an SM share its shared memory");
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // The clusters that fit the device at once take equal runs; one more would start when the
+  // others are done. (Groups of SMs that hold no whole number of clusters leave slots empty.)
+  static std::atomic<int> fit[kKV8MaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kKV8MaxDevices) return cudaErrorInvalidDevice;
+  int n = fit[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = kKV8CL;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kKV8CL);
+    cfg.blockDim = dim3(kKV8Warps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&n, k, &cfg);
+    if (e != cudaSuccess) return e;
+    n = n < 1 ? 1 : n;
+    fit[dev].store(n, std::memory_order_relaxed);
+  }
+  a.clusters = n < a.clusters ? n : a.clusters;
   return hx_launch_pdl_cluster(k, dim3((unsigned)(a.clusters * kKV8CL)), dim3(kKV8Warps * 32), smem, st, kKV8CL, a);
 }
 

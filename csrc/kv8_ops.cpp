@@ -157,8 +157,8 @@ void attn_decode_kv8(torch::Tensor proj, c10::optional<torch::Tensor> q_norm_w, 
                   proj.size(1) >= Hq * qw + 2 * Hkv * D,
               "proj bf16 [B, q (+ gate) | k | v]");
   TORCH_CHECK(out.scalar_type() == at::kBFloat16 && out.is_contiguous() && out.dim() == 2 && out.size(0) == B &&
-                  out.size(1) == Hq * D,
-              "out bf16 [B, Hq * D]");
+                  out.size(1) == Hq * D && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+              "out bf16 [B, Hq * D], 16-byte aligned");
   TORCH_CHECK(rot >= 0 && rot <= D && rot % 2 == 0, "rotary dims: even, at most the head dim");
   TORCH_CHECK(inv_freq.scalar_type() == at::kFloat && inv_freq.is_contiguous() && inv_freq.numel() >= rot / 2,
               "inv_freq f32 [rot/2]");
@@ -170,6 +170,7 @@ void attn_decode_kv8(torch::Tensor proj, c10::optional<torch::Tensor> q_norm_w, 
   TORCH_CHECK(B <= kKV8MaxBatch, "at most ", kKV8MaxBatch, " sequences");
   a.NT = kv8_tiles((int)(Hq / Hkv), (int)D);
   a.HG = kv8_groups((int)(Hq / Hkv), (int)D);
+  TORCH_CHECK((double)B * Hkv * a.HG * a.c.nb < 2e9, "more than 2^31 blocks to attend to");
   a.clusters = kv8_clusters(kc.device().index());
   TORCH_CHECK(ws.scalar_type() == at::kInt && ws.is_contiguous() &&
                   ws.numel() >= kv8_ws_words(a.clusters, B * Hkv * a.HG, D, a.NT),
