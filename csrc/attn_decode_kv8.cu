@@ -56,6 +56,7 @@ struct DecodeKV8Smem {
   alignas(16) uint2 qf[NT][D / 16][32];  // the same as f16 operands, a lane's four values together
   alignas(16) __nv_bfloat16 knew[D], vnew[D];  // the new token as the cache holds it
   float ps[kKV8Warps][2 * NT][32][4];    // the warps' parts of the last block's scores
+  float wq[D], wk[D];                    // norm weights
   float cs[D / 2], sn[D / 2];            // rotation of the sequence's position
   float qmul[GP];                        // score factor of each head: scale * log2(e) / power of two
   float wm[kKV8Warps][GP], wl[kKV8Warps][GP];
@@ -65,7 +66,7 @@ struct DecodeKV8Smem {
   int off[kKV8MaxBatch + 1];             // blocks before sequence b
   int slot[kKV8MaxBatch], pos[kKV8MaxBatch];
   int nbmax;
-  float red[2][kKV8Warps];
+  float red[2][kKV8Warps], inv[2], scale[2];
   int last;
 };
 
@@ -74,6 +75,20 @@ HX_DEVICE void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 2^x to 2 ulp, 0 below 2^-126.
+HX_DEVICE float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// sin and cos of an f32 angle. The turns are taken off in f64, so the argument left is exact to
+// 2^-24 of a turn at any position.
+HX_DEVICE void rotation(float angle, float* sn, float* cs) {
+  const double turns = (double)angle * 0.15915494309189535;
+  sincospif((float)(2.0 * (turns - rint(turns))), sn, cs);
 }
 
 HX_DEVICE uint32_t movmatrix_t(uint32_t x) {
@@ -173,11 +188,20 @@ struct DecodeKV8Warp {
   // O^T += V^T . P over the 64 dims of panel u (64 dims x 32 codes in shared memory)
   HX_DEVICE void pv_panel(const uint8_t* p, int u, float vs) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pv_tile(p, i, u * 4 + i, vs);
+    for (int i = 0; i < 4; ++i) {
+      float o[NT][4];
+      pv_tile(p, i, o);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float (&c)[4] = acc[u * 4 + i][nt];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = fmaf(c[e], corr[nt][e & 1], o[nt][e] * vs);
+      }
+    }
   }
 
-  // dims 16 i .. 16 i + 15 of a panel, output tile `to`
-  HX_DEVICE void pv_tile(const uint8_t* p, int i, int to, float vs) {
+  // o[nt] = V^T . P of dims 16 i .. 16 i + 15 of a panel, in codes
+  HX_DEVICE void pv_tile(const uint8_t* p, int i, float (&o)[NT][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint2 x = *reinterpret_cast<const uint2*>(p + (i * 16 + g) * 32 + t * 8);
     const uint2 y = *reinterpret_cast<const uint2*>(p + (i * 16 + g + 8) * 32 + t * 8);
@@ -188,12 +212,9 @@ struct DecodeKV8Warp {
     codes_to_f16<FP8>(y.y, a[1][1], a[1][3]);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float o[4] = {0.f, 0.f, 0.f, 0.f};
+      o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) mma_f16(o, a[s][0], a[s][1], a[s][2], a[s][3], pb[s][nt][0], pb[s][nt][1]);
-      float (&c)[4] = acc[to][nt];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c[e] = fmaf(c[e], corr[nt][e & 1], o[e] * vs);
+      for (int s = 0; s < 2; ++s) mma_f16(o[nt], a[s][0], a[s][1], a[s][2], a[s][3], pb[s][nt][0], pb[s][nt][1]);
     }
   }
 
@@ -219,15 +240,14 @@ struct DecodeKV8Warp {
         for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         const float mn = fmaxf(m[nt][e], mx);
         const float base = mn == -INFINITY ? 0.f : mn - 8.f;
-        corr[nt][e] = exp2f(m[nt][e] - mn);
-        if (m[nt][e] == -INFINITY) corr[nt][e] = 0.f;
+        corr[nt][e] = m[nt][e] == -INFINITY ? 0.f : exp2_fast(m[nt][e] - mn);
         float sum = 0.f;
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             float& x = sc[s][nt][2 * j + e];
-            x = exp2f(x - base);
+            x = exp2_fast(x - base);
             sum += x;
           }
         l[nt][e] = fmaf(l[nt][e], corr[nt][e], sum);
@@ -277,14 +297,24 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
   }
   pdl_wait_prior();
   pdl_launch_dependents();
+  for (int d = tid; d < D; d += NTH) {
+    s->wq[d] = a.q_norm_w ? a.q_norm_w[d] : 1.f;
+    s->wk[d] = a.k_norm_w ? a.k_norm_w[d] : 1.f;
+  }
+  const float freq = tid < a.rot / 2 ? a.inv_freq[tid] : 0.f;
+  static_assert(D / 2 <= NTH, "a thread for each rotary frequency");
   // ---- blocks of each sequence (0: refused), and the blocks before it -------------------------
   if (warp == 0) {
     int base = 0, most = 0;
+    const int first = lane < a.c.S ? a.pos[lane] : -1;  // of slots 0..31, fetched with the slot ids
+#pragma unroll 1
     for (int b0 = 0; b0 < a.B; b0 += 32) {
       int n = 0;
+      const int slot = b0 + lane < a.B ? a.slots[b0 + lane] : -1;
+      int p = __shfl_sync(0xffffffffu, first, slot & 31);
+      if (slot < 0 || slot >= a.c.S) p = -1;
+      else if (slot >= 32) p = a.pos[slot];
       if (b0 + lane < a.B) {
-        const int slot = a.slots[b0 + lane];
-        const int p = slot >= 0 && slot < a.c.S ? a.pos[slot] : -1;
         n = p >= 0 && p < a.c.nb * kKV8Block ? p / kKV8Block + 1 : 0;
         s->slot[b0 + lane] = slot;
         s->pos[b0 + lane] = p;
@@ -322,7 +352,8 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
   const int wend = min(W - w, chunk) + w;
   float* part_o = reinterpret_cast<float*>(a.ws + kKV8PartAt);  // [NC + pairs][GP][D]
   float2* part_ml = reinterpret_cast<float2*>(part_o + (long long)(NC + a.B * PB) * GP * D);  // [NC + pairs][GP]
-  unsigned seq = 0;  // copies this warp has issued in all
+  int put = 0, get = 0;  // ring slots of the next copy issued (lane 0) and used
+  uint32_t phase = 0;    // parity of the slot to use next
   bool ok = true;
   DecodeKV8Warp<D, NT, FP8> st;
   int b = 0;
@@ -349,26 +380,31 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
     const bool cta_last = blk1 == nb && (nb - 1 - blk0) % (CL * NW) / NW == crank;
     const bool completes = cta_last && row == kKV8Block - 1;
     const int host = (nb - 1 - blk0) % NW;  // the warp whose ring holds the codes of a completed block
-    const unsigned units = (unsigned)mine * 2 * R::kUK;
-    const uint8_t* kbase = a.c.kc + a.c.block(slot, h, 0) * (D * kKV8Block);
-    const uint8_t* vbase = a.c.vc + a.c.block(slot, h, 0) * (D * kKV8Block);
-    auto issue = [&](unsigned i) {  // lane 0: unit i of this segment
-      const unsigned sl = (seq + i) % R::kSlots, in = i % (2 * R::kUK);
-      const long long blk = my0 + (long long)(i / (2 * R::kUK)) * (CL * NW);
-      const uint8_t* src = (in < R::kUK ? kbase : vbase) + blk * (D * kKV8Block) + (in % R::kUK) * R::kUnit;
-      tc::mbar_expect_tx(&s->full[warp][sl], R::kUnit);
-      bulk_load(s->ring[warp][sl], src, R::kUnit, &s->full[warp][sl]);
+    // lane 0 copies unit after unit: K then V of a block, block after block
+    int todo = mine * 2 * R::kUK, in = 0;
+    const uint8_t* kp = a.c.kc + a.c.block(slot, h, my0) * (D * kKV8Block);
+    const uint8_t* vp = a.c.vc + a.c.block(slot, h, my0) * (D * kKV8Block);
+    auto issue = [&] {
+      const uint8_t* src = in < R::kUK ? kp + in * R::kUnit : vp + (in - R::kUK) * R::kUnit;
+      tc::mbar_expect_tx(&s->full[warp][put], R::kUnit);
+      bulk_load(s->ring[warp][put], src, R::kUnit, &s->full[warp][put]);
+      if (++in == 2 * R::kUK) {
+        in = 0;
+        kp += (long long)CL * NW * D * kKV8Block;
+        vp += (long long)CL * NW * D * kKV8Block;
+      }
+      put = put + 1 == R::kSlots ? 0 : put + 1;
+      --todo;
     };
     auto fill = [&] {
-      if (lane == 0 && ok)
-        for (unsigned i = 0; i < min(units, (unsigned)R::kSlots); ++i) issue(i);
+#pragma unroll 1
+      for (int i = 0; i < R::kSlots && todo > 0 && ok && lane == 0; ++i) issue();
     };
     if (!(completes && warp == host)) fill();
     // ---- loads of all that the segment's start needs, in flight together -------------------------
     const int nrow = n + (cta_last ? 1 : 0);  // the group's queries, then the new key
     constexpr int NR = (GP + NW) / NW;
     __nv_bfloat16 xr[NR][D / 32], xv[D / 32];
-    float wq[D / 32], wk[D / 32];
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const int r = warp + i * NW;
@@ -378,12 +414,9 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         for (int e = 0; e < D / 32; ++e) xr[i][e] = src[e * 32 + lane];
     }
     const bool kwarp = cta_last && warp == n % NW;
+    if (kwarp)
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      wq[e] = a.q_norm_w ? a.q_norm_w[e * 32 + lane] : 1.f;
-      wk[e] = kwarp && a.k_norm_w ? a.k_norm_w[e * 32 + lane] : 1.f;
-      if (kwarp) xv[e] = pr[a.Hq * qw + (Hkv + h) * D + e * 32 + lane];
-    }
+      for (int e = 0; e < D / 32; ++e) xv[e] = pr[a.Hq * qw + (Hkv + h) * D + e * 32 + lane];
     // The last block's bf16 rows, for the whole CTA: for a completed block 16-value pieces of the
     // block's layout (X[i][0..1] of K, [2..3] of V); else operands: warp w takes dims groups
     // (of 16) w * NP + i of the sums and of the output.
@@ -413,7 +446,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       }
     }
     const int prot = p + (a.rope_delta ? a.rope_delta[slot] : 0);
-    for (int i = tid; i < a.rot / 2; i += NTH) sincosf((float)prot * a.inv_freq[i], &s->sn[i], &s->cs[i]);
+    if (const int i = tid; i < a.rot / 2) rotation((float)prot * freq, &s->sn[i], &s->cs[i]);
     __syncthreads();
     // ---- q of the group's heads (and the new key): norm, rotation ------------------------------
 #pragma unroll
@@ -431,7 +464,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       if (isk ? a.k_norm_w : a.q_norm_w) {
         const float inv = rsqrtf(warp_sum(ss) / D + a.eps);
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) v[e] *= inv * (isk ? wk[e] : wq[e]);
+        for (int e = 0; e < D / 32; ++e) v[e] *= inv * (isk ? s->wk : s->wq)[e * 32 + lane];
       }
       const int half = a.rot / 2;
       if (half) {
@@ -470,7 +503,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
           const int k = (d >> 6) * 4 + ((d >> 2) & 3), l = (r & 7) * 4 + ((d >> 4) & 3);
           qf[(k * 32 + l) * 4 + (d & 3)] = __float2half_rn(v[e] * up);
         }
-        if (lane == 0) s->qmul[r] = a.sl2 / up;
+        if (lane == 0) s->qmul[r] = a.sl2 * __uint_as_float((uint32_t)(127 - ex) << 23);
       }
     }
     __syncthreads();
@@ -526,11 +559,19 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         }
         __syncthreads();
         const long long at = a.c.block(slot, h, nb - 1);
+        if (tid < 2) {
+          const float m = fmaxf(fmaxf(s->red[tid][0], s->red[tid][1]), fmaxf(s->red[tid][2], s->red[tid][3]));
+          const float scale = kv8_scale<FP8>(m);
+          s->inv[tid] = kv8_inv<FP8>(m);
+          s->scale[tid] = scale;
+          if (hg == 0) (tid ? a.c.vs : a.c.ks)[at] = scale;
+        }
+        __syncthreads();
+        ksc = s->scale[0];
+        vsc = s->scale[1];
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          const float m = fmaxf(fmaxf(s->red[z][0], s->red[z][1]), fmaxf(s->red[z][2], s->red[z][3]));
-          const float inv = kv8_inv<FP8>(m);
-          (z ? vsc : ksc) = kv8_scale<FP8>(m);
+          const float inv = s->inv[z];
           uint8_t* dst = (z ? a.c.vc : a.c.kc) + at * (D * kKV8Block);
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
@@ -542,7 +583,6 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
             reinterpret_cast<uint4*>(fresh + z * D * kKV8Block)[i * NTH + tid] = v;
             if (hg == 0) reinterpret_cast<uint4*>(dst)[i * NTH + tid] = v;
           }
-          if (hg == 0 && tid == 0) (z ? a.c.vs : a.c.ks)[at] = z ? vsc : ksc;
         }
         __syncthreads();
 #pragma unroll
@@ -612,16 +652,13 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       if (warp != 0)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) st.l[nt][0] = st.l[nt][1] = 0.f;
+      float own[NP][NT][4];  // this warp's dims of the output
       if (completes) {
         st.pack_p();
 #pragma unroll
-        for (int q = 0; q < NP; ++q) {
-          const uint8_t* src = fresh + D * kKV8Block + q * kKV8Panel;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if ((q * 4 + i) / NP != warp) continue;
-            st.pv_tile(src, i, q * 4 + i, vsc);
-          }
+        for (int i = 0; i < NP; ++i) {
+          const int k = warp * NP + i;
+          st.pv_tile(fresh + D * kKV8Block + (k >> 2) * kKV8Panel, k & 3, own[i]);
         }
       } else {
         uint32_t ph[2][NT][2], pl2[2][NT][2];
@@ -650,14 +687,15 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
           }
         };
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          if (i / NP != warp) continue;
+        for (int i = 0; i < NP; ++i) {
+          const int k = warp * NP + i;
           uint32_t x[4], y[4];
-          clean(i * 16 + g, X[i % NP][2], x);
-          clean(i * 16 + g + 8, X[i % NP][3], y);
+          clean(k * 16 + g, X[i][2], x);
+          clean(k * 16 + g + 8, X[i][3], y);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float (&o)[4] = st.acc[i][nt];  // still zero: this block is the first
+            float (&o)[4] = own[i][nt];
+            o[0] = o[1] = o[2] = o[3] = 0.f;
 #pragma unroll
             for (int sx = 0; sx < 2; ++sx) {
               mma_16816(o, x[2 * sx], y[2 * sx], x[2 * sx + 1], y[2 * sx + 1], ph[sx][nt][0], ph[sx][nt][1]);
@@ -666,6 +704,13 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
           }
         }
       }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)  // this block is the first: the sums start with it
+        if (i / NP == warp)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st.acc[i][nt][e] = own[i % NP][nt][e] * vsc;
       if (completes) {
         __syncthreads();  // every warp is done with the codes
         if (warp == host) {
@@ -678,19 +723,29 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
     // ---- complete blocks -----------------------------------------------------------------------
     const float* ksp = a.c.ks + a.c.block(slot, h, 0);
     const float* vsp = a.c.vs + a.c.block(slot, h, 0);
-    unsigned u = 0;
-    auto next_unit = [&](auto&& use) {  // wait for unit u, use it, hand its slot to unit u + kSlots
-      const unsigned sl = (seq + u) % R::kSlots;
-      if (ok) ok = tc::mbar_wait(&s->full[warp][sl], ((seq + u) / R::kSlots) & 1, a.ws, 6002);
+    auto next_unit = [&](auto&& use) {  // wait for a unit, use it, hand its slot to a later one
+      if (ok) ok = tc::mbar_wait(&s->full[warp][get], phase, a.ws, 6002);
       ok = __all_sync(0xffffffffu, ok);
-      use(s->ring[warp][sl]);
+      use(s->ring[warp][get]);
       __syncwarp();
-      if (lane == 0 && ok && u + R::kSlots < units) issue(u + R::kSlots);
-      ++u;
+      if (lane == 0 && ok && todo > 0) issue();
+      if (++get == R::kSlots) {
+        get = 0;
+        phase ^= 1;
+      }
     };
+    float ks = 0.f, vs = 0.f;
+    if (mine > 0) {
+      ks = __ldcg(ksp + my0);
+      vs = __ldcg(vsp + my0);
+    }
+#pragma unroll 1
     for (int i = 0; i < mine && ok; ++i) {
-      const int blk = my0 + i * (CL * NW);
-      const float ks = __ldcg(ksp + blk), vs = __ldcg(vsp + blk);
+      const float ks0 = ks, vs0 = vs;
+      if (i + 1 < mine) {  // the next block's scales are under way meanwhile
+        ks = __ldcg(ksp + my0 + (i + 1) * (CL * NW));
+        vs = __ldcg(vsp + my0 + (i + 1) * (CL * NW));
+      }
       st.clear_scores();
 #pragma unroll
       for (int k = 0; k < R::kUK; ++k)
@@ -698,17 +753,16 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
 #pragma unroll
           for (int q = 0; q < R::kUnit / kKV8Panel; ++q) st.qk_panel(x + q * kKV8Panel, k * (R::kUnit / kKV8Panel) + q);
         });
-      st.softmax(ks, kKV8Block);
+      st.softmax(ks0, kKV8Block);
       st.pack_p();
 #pragma unroll
       for (int k = 0; k < R::kUK; ++k)
         next_unit([&](const uint8_t* x) {
 #pragma unroll
           for (int q = 0; q < R::kUnit / kKV8Panel; ++q)
-            st.pv_panel(x + q * kKV8Panel, k * (R::kUnit / kKV8Panel) + q, vs);
+            st.pv_panel(x + q * kKV8Panel, k * (R::kUnit / kKV8Panel) + q, vs0);
         });
     }
-    seq += units;
     // ---- merge the warps: the ring's memory holds their O now --------------------------------------
     __syncthreads();
 #pragma unroll
@@ -730,6 +784,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
 #pragma unroll
         for (int c = 0; c < 4; ++c) s->wo[warp][nt * 8 + 2 * t + (c & 1)][i * 16 + g + (c >> 1) * 8] = st.acc[i][nt][c];
     __syncthreads();
+#pragma unroll 1
     for (int i = tid; i < n * (D / 4); i += NTH) {  // four dims of one head
       const int r = i / (D / 4), d = i % (D / 4) * 4;
       float M = -INFINITY, L = 0.f;
@@ -738,7 +793,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       for (int x = 0; x < NW; ++x) M = fmaxf(M, s->wm[x][r]);
 #pragma unroll
       for (int x = 0; x < NW; ++x) {
-        const float f = s->wm[x][r] == -INFINITY ? 0.f : exp2f(s->wm[x][r] - M);
+        const float f = s->wm[x][r] == -INFINITY ? 0.f : exp2_fast(s->wm[x][r] - M);
         add4(O, *reinterpret_cast<const float4*>(&s->wo[x][r][d]), f);
         L = fmaf(s->wl[x][r], f, L);
       }
@@ -749,11 +804,12 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
     cluster.sync();
     auto finish = [&](int r, int d, float4 o, float l) {  // four dims of the output
       const int hq = h * G + g0 + r;
-      float f[4] = {o.x / l, o.y / l, o.z / l, o.w / l};
+      const float il = __fdividef(1.f, l);
+      float f[4] = {o.x * il, o.y * il, o.z * il, o.w * il};
       if (a.gated) {
         const __nv_bfloat16* gp = pr + (long long)hq * qw + D + d;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = f[e] / (1.f + __expf(-__bfloat162float(gp[e])));
+        for (int e = 0; e < 4; ++e) f[e] = __fdividef(f[e], 1.f + __expf(-__bfloat162float(gp[e])));
       }
       uint2 y;
       y.x = pack_bf16x2(f[0], f[1]);
@@ -762,6 +818,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
     };
     const bool alone = blk0 == 0 && blk1 == nb;
     const int cols = n * (D / 4) / CL, c0 = crank * cols;  // in fours
+#pragma unroll 1
     for (int i = c0 + tid; i < c0 + cols; i += NTH) {
       const int r = i / (D / 4), d = i % (D / 4) * 4;
       float m[CL], l[CL], M = -INFINITY, L = 0.f;
@@ -776,7 +833,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       for (int x = 0; x < CL; ++x) M = fmaxf(M, m[x]);
 #pragma unroll
       for (int x = 0; x < CL; ++x) {
-        const float f = m[x] == -INFINITY ? 0.f : exp2f(m[x] - M);
+        const float f = m[x] == -INFINITY ? 0.f : exp2_fast(m[x] - M);
         L = fmaf(l[x], f, L);
         add4(O, v[x], f);
       }
@@ -805,6 +862,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         const int f0 = p0 / chunk, np = (p0 + nb - 1) / chunk - f0 + 1;  // its clusters
         const long long q0 = f0 + pair;
         const int r0 = c0 / (D / 4), r1 = (c0 + cols - 1) / (D / 4);       // heads of this CTA's columns
+#pragma unroll 1
         for (int r = r0 + warp; r <= r1; r += NW) {
           constexpr int NX = (kKV8MaxPart + 31) / 32;
           float2 ml[NX];
@@ -817,7 +875,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
           M = warp_max(M);
 #pragma unroll
           for (int x = 0; x < NX; ++x) {
-            const float f = ml[x].x == -INFINITY ? 0.f : exp2f(ml[x].x - M);
+            const float f = ml[x].x == -INFINITY ? 0.f : exp2_fast(ml[x].x - M);
             if (x * 32 + lane < np) s->fw[r][x * 32 + lane] = f;
             L = fmaf(ml[x].y, f, L);
           }
@@ -825,9 +883,11 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
           if (lane == 0) s->lsum[r] = L;
         }
         __syncthreads();
+#pragma unroll 1
         for (int i = c0 + tid; i < c0 + cols; i += NTH) {
           const int r = i / (D / 4), d = i % (D / 4) * 4;
           float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
           for (int x = 0; x < np; x += 16) {  // sixteen loads in flight
             float4 v[16];
 #pragma unroll
