@@ -26,6 +26,7 @@
 #include <atomic>
 
 #include "kv8.cuh"
+#include "kv8_f16.cuh"
 #include "mma_frag.cuh"
 #include "tc_common.cuh"
 
@@ -77,13 +78,6 @@ HX_DEVICE void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 2^x to 2 ulp, 0 below 2^-126.
-HX_DEVICE float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // sin and cos of an f32 angle. The turns are taken off in f64, so the argument left is exact to
 // 2^-24 of a turn at any position.
 HX_DEVICE void rotation(float angle, float* sn, float* cs) {
@@ -102,31 +96,6 @@ HX_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* b
                    tc::smem_u32(dst)),
                "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
                : "memory");
-}
-
-HX_DEVICE uint32_t pack_f16x2(float lo, float hi) {
-  __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-
-// Four codes -> two f16 pairs, exactly. int8: a byte offset by 128 under the exponent of 1024
-// is 1024 + code + 128.
-template <bool FP8>
-HX_DEVICE void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (FP8) {
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffff), __NV_E4M3);
-    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-    lo = *reinterpret_cast<const uint32_t*>(&a);
-    hi = *reinterpret_cast<const uint32_t*>(&b);
-  } else {
-    const uint32_t u = w ^ 0x80808080u;
-    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    const uint32_t bias = 0x64806480u;  // 1152
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&bias));
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&bias));
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  }
 }
 
 // The key that row r (0..7) of score tile (s, j) holds. P's tiles then transpose into operands

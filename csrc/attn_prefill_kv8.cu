@@ -1,44 +1,562 @@
-// Causal GQA attention of a prompt's tokens over the 8-bit KV cache (kv8.cuh).
+// Causal GQA attention of a prompt's tokens over the 8-bit KV cache (kv8.cuh), on tcgen05.
 //
 // o[t, h, :] = softmax_j(q[t, h] . k[j, h / G] * scale, j <= p0 + t) v[j, h / G]  [* sigmoid(gate)]
 // for T tokens at positions p0 .. p0+T-1 whose keys and values are already in the cache.
-#include "attn_kv8.cuh"
+//
+// A CTA takes NT tiles of 128 query rows of one kv head; row r is token r / G, query head r % G,
+// so the G heads that share K / V share every tile of it. Codes are exact in f16: K and V enter
+// the tensor cores as f16 codes and the blocks' scales stay f32 factors outside:
+//   s_j = (q . c_j) ks_b,   p'_j = 2^(s_j - m) (vs_b / vref),   o = vref sum_j p'_j c'_j / l
+// with vs_b / vref added in the exponent (no extra work for a key) and vref the largest V scale
+// that the CTA sees. The incomplete last block is bf16: it is brought to f16 after a power of two
+// that takes its largest entry to 128..256. So is every row of q (11 bits stay, entries 2^32
+// below the row's largest vanish).
+//
+//   warps 0-3        converters: 8-bit panels from global memory -> f16 tiles of BN keys in shared
+//                    memory, in the 128-byte-swizzled layout the MMA reads (2-stage rings for K, V);
+//   next 4 NT warps  softmax, a thread a row: scores from TMEM, running max with a lazy rescale of O
+//                    (only when the max grows by more than 2^8), P as f16 back into the score
+//                    columns of TMEM, from where it is the A operand of P V;
+//   last warp        issues the MMAs from one thread. Score buffers alternate (the two tiles', or
+//                    two of one tile), so the tensor cores work on one while the other is in softmax.
+// With few rows the keys are split over CTAs and their (O, max, sum) merged by a second kernel.
+// Every wait is bounded (error code 7000 + site); on expiry the CTA stops and frees its TMEM.
+#include <cuda_fp16.h>
+
+#include "kv8.cuh"
+#include "kv8_f16.cuh"
+#include "tc_common.cuh"
 
 namespace hx {
 
-template <int D, bool FP8>
-__global__ void __launch_bounds__(128) attn_prefill_kv8_kernel(AttnPrefillKV8Args a) {
-  extern __shared__ __align__(16) unsigned char raw[];
-  auto* s = reinterpret_cast<KV8RowsSmem<D>*>(raw);
-  constexpr int ND = (D + 127) / 128;
+// ---- TMEM --------------------------------------------------------------------------------------
+// 64 consecutive f32 columns of this thread's lane; the loads and their wait are one statement, so
+// nothing that uses the values can be scheduled between them.
+HX_DEVICE void tmem_ld64(uint32_t taddr, float* v) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,"
+      "%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+HX_DEVICE void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+HX_DEVICE void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[smem] * B[smem]^T and D[tmem] (+)= A[tmem] * B[smem]^T, f16 inputs, f32 accumulate.
+HX_DEVICE void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+HX_DEVICE void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+HX_DEVICE constexpr uint32_t idesc_f16_f32(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);  // f32 accumulator, f16 A and B
+}
+
+// A power of two that takes a largest magnitude to 128..256, and its inverse (zero stays as it is).
+HX_DEVICE void pow2_scale(float mag, float* up, float* down) {
+  const int ex = min(134 - (int)(__float_as_uint(mag) >> 23), 120);
+  *up = __uint_as_float((uint32_t)(ex + 127) << 23);
+  *down = __uint_as_float((uint32_t)(127 - ex) << 23);
+}
+
+// Gate and store 16 dims from d0 of a row.
+HX_DEVICE void finish16(const AttnPrefillKV8Args& a, int t, int hq, int d0, float* o) {
+  if (a.gate) {
+    float g[16];
+    load16(a.gate + t * a.ldg_t + hq * a.ldg_h, d0, a.vec_g, g);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = __fdividef(o[e], 1.f + __expf(-g[e]));
+  }
+  __nv_bfloat16* dst = a.o + t * a.ldo + (long long)hq * (a.c.D) + d0;
+  if (a.vec_o) {
+    reinterpret_cast<bf16x8*>(dst)[0] = pack8(o);
+    reinterpret_cast<bf16x8*>(dst)[1] = pack8(o + 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dst[e] = __float2bfloat16(o[e]);
+  }
+}
+
+template <int D, int NT, int BN>
+struct PrefillKV8Smem {
+  alignas(1024) __half Q[NT][128 * D];  // per tile: D/64 chunks of [128 rows x 64], 128B-swizzled
+  alignas(1024) __half K[2][BN * D];    // per stage: D/64 chunks of [BN keys x 64 dims]
+  alignas(1024) __half V[2][BN * D];    // per stage: BN/64 chunks of [D dims x 64 keys]
+  float kmul[4][BN / 32];               // tile j at j % 4: score factor of each 32 keys,
+  float vadd[4][BN / 32];               // log2(vs / vref) and its inverse factor
+  float vinv[4][BN / 32];
+  float red[3][16];
+  float tail[4];                        // K tail: up, down; V tail: up, down
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[4], s_full[2], p_full[2], o_done[NT];
+  uint32_t tmem_base;
+  int abort;
+};
+
+template <int D, int NT, int BN, bool FP8>
+__global__ void __launch_bounds__(160 + 128 * NT, 1) attn_prefill_kv8_kernel(AttnPrefillKV8Args a) {
+  static_assert(NT * D + 2 * BN <= 512, "TMEM: the tiles' O and two score buffers");
+  using SM = PrefillKV8Smem<D, NT, BN>;
+  constexpr int NTH = 160 + 128 * NT, MMA_WARP = 4 + 4 * NT, NG = BN / 32, NP = D / 64;
+  constexpr uint32_t S_COL = NT * D;
+  extern __shared__ __align__(1024) unsigned char raw[];
+  SM* s = reinterpret_cast<SM*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int h = blockIdx.x, G = a.Hq / a.c.Hkv, R = a.T * G, L = a.p0 + a.T, nf = L / kKV8Block;
+  const int r0 = (gridDim.y - 1 - blockIdx.y) * 128 * NT;  // the longest rows first
+  const int kend = a.p0 + (min(r0 + 128 * NT, R) - 1) / G + 1;  // keys that any of the CTA's rows sees
+  const int nball = (kend + BN - 1) / BN, per = (nball + gridDim.z - 1) / gridDim.z;
+  const int jb = blockIdx.z * per, nb = max(0, min(nball, jb + per) - jb);  // this split's tiles
+
+  if (tid == 0) {
+    tc::mbar_init(&s->q_full, 4 * NT);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&s->k_full[i], 4);
+      tc::mbar_init(&s->k_empty[i], 1);
+      tc::mbar_init(&s->v_full[i], 4);
+      tc::mbar_init(&s->v_empty[i], 1);
+      tc::mbar_init(&s->s_full[i], 1);
+      tc::mbar_init(&s->p_full[i], 4);
+    }
+    for (int i = 0; i < 4; ++i) tc::mbar_init(&s->sc_full[i], 1);
+    for (int i = 0; i < NT; ++i) tc::mbar_init(&s->o_done[i], 1);
+    s->abort = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == MMA_WARP) {
+    tc::tmem_alloc(&s->tmem_base, 512);
+    tc::tmem_relinquish();
+  }
   pdl_wait_prior();
   pdl_launch_dependents();
-  const int t0 = blockIdx.x * kKV8Rows, hq = blockIdx.y, h = hq / (a.Hq / a.c.Hkv), tid = threadIdx.x;
-  const int n = min(kKV8Rows, a.T - t0);
-  for (int i = tid; i < n * D; i += 128)
-    s->q[i / D][i % D] = __bfloat162float(a.q[(t0 + i / D) * a.ldq + hq * D + i % D]) * a.sl2;
-  float acc[kKV8Rows][ND];
-  attend_rows<D, FP8>(a.c, a.slot, h, a.p0 + a.T, n, [&](int r) { return a.p0 + t0 + r + 1; }, s, acc);
-#pragma unroll
-  for (int r = 0; r < kKV8Rows; ++r)
-#pragma unroll
-    for (int i = 0; i < ND; ++i) {
-      const int d = tid + 128 * i;
-      if (r >= n || d >= D) continue;
-      float o = acc[r][i];
-      if (a.gate) o = o / (1.f + __expf(-__bfloat162float(a.gate[(t0 + r) * a.ldg_t + hq * a.ldg_h + d])));
-      a.o[(t0 + r) * a.ldo + hq * D + d] = __float2bfloat16(o);
+  // ---- the largest V scale in sight, and the tail's scales ---------------------------------------
+  const uint8_t* kc = a.c.kc + a.c.block(a.slot, h, 0) * (D * kKV8Block);
+  const uint8_t* vc = a.c.vc + a.c.block(a.slot, h, 0) * (D * kKV8Block);
+  const float* ks = a.c.ks + a.c.block(a.slot, h, 0);
+  const float* vs = a.c.vs + a.c.block(a.slot, h, 0);
+  const __nv_bfloat16* kt = a.c.kt + a.c.head(a.slot, h) * (D * kKV8Block);
+  const __nv_bfloat16* vt = a.c.vt + a.c.head(a.slot, h) * (D * kKV8Block);
+  const int tl = kend > nf * kKV8Block ? L - nf * kKV8Block : 0;  // tail rows that this CTA reads
+  {
+    float mv = 0.f, mk = 0.f, mt = 0.f;
+    for (int i = tid; i < min(nf, (kend + kKV8Block - 1) / kKV8Block); i += NTH) mv = fmaxf(mv, vs[i]);
+    if (tl)
+      for (int i = tid; i < D * kKV8Block; i += NTH) {
+        if (i % kKV8Panel / 64 < tl) mk = fmaxf(mk, kv8_mag(__bfloat162float(kt[i])));
+        if (i % kKV8Block < tl) mt = fmaxf(mt, kv8_mag(__bfloat162float(vt[i])));
+      }
+    mv = warp_max(mv);
+    mk = warp_max(mk);
+    mt = warp_max(mt);
+    if (lane == 0) { s->red[0][warp] = mv; s->red[1][warp] = mk; s->red[2][warp] = mt; }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  float vref = 0.f;
+  {
+    float mk = 0.f, mt = 0.f;
+    for (int w = 0; w < NTH / 32; ++w) {
+      vref = fmaxf(vref, s->red[0][w]);
+      mk = fmaxf(mk, s->red[1][w]);
+      mt = fmaxf(mt, s->red[2][w]);
     }
+    if (tl && tid == 0) {
+      pow2_scale(mk, &s->tail[0], &s->tail[1]);
+      pow2_scale(mt, &s->tail[2], &s->tail[3]);
+    }
+    float up, down;
+    pow2_scale(mt, &up, &down);
+    if (mt > 0.f) vref = fmaxf(vref, down);
+    if (!(vref > 0.f)) vref = 1.f;
+  }
+  __syncthreads();
+  const uint32_t tmem = s->tmem_base;
+
+  if (warp < 4) {
+    // ------------------------------------ converters ---------------------------------------------
+    // A piece is 16 codes (32 bytes of f16): for K 16 dims of a key, for V 16 keys of a dim. Four
+    // neighbouring lanes hold one 128-byte row of a chunk, so stores meet no bank twice.
+    constexpr int PC = BN * D / 16 / 128;  // pieces of a thread
+    const int row8 = lane >> 2, part = lane & 3;
+    bool ok = true;
+    uint4 xk[PC], xv[PC];
+    // piece i: eight rows (warp + 4 i) * 8 .. + 7 of the tile's chunks
+    auto load = [&](int j, bool isv, uint4 (&x)[PC]) {
+#pragma unroll
+      for (int i = 0; i < PC; ++i) {
+        const int rw = (warp + 4 * i) * 8 + row8;        // row over all chunks
+        if (!isv) {
+          const int c = rw / BN, key = rw % BN, b = j * NG + key / 32;
+          if (b < nf) x[i] = __ldg(reinterpret_cast<const uint4*>(kc + ((long long)b * NP + c) * kKV8Panel + (key % 32) * 64 + part * 16));
+        } else {
+          const int c = rw / D, dim = rw % D, b = j * NG + c * 2 + (part >> 1);
+          if (b < nf) x[i] = __ldg(reinterpret_cast<const uint4*>(vc + (long long)b * (D * kKV8Block) + dim * 32 + (part & 1) * 16));
+        }
+      }
+    };
+    auto store = [&](int j, bool isv, const uint4 (&x)[PC], __half* dst) {
+#pragma unroll
+      for (int i = 0; i < PC; ++i) {
+        const int rw = (warp + 4 * i) * 8 + row8;
+        const int key = isv ? 0 : rw % BN, c = isv ? rw / D : 0, dim = isv ? rw % D : 0;
+        const int b = isv ? j * NG + c * 2 + (part >> 1) : j * NG + key / 32;
+        uint32_t y[8];
+        if (b < nf) {
+          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) codes_to_f16<FP8>(w[e], y[2 * e], y[2 * e + 1]);
+        } else {  // the tail, or past the sequence: zeros there (their probabilities are zero as well)
+          const float up = s->tail[isv ? 2 : 0];
+#pragma unroll 1
+          for (int e = 0; e < 8; ++e) {
+            float f[2];
+            for (int q = 0; q < 2; ++q) {
+              const int el = part * 16 + e * 2 + q;
+              bool in;
+              float val = 0.f;
+              if (isv) {
+                const int kk = (part & 1) * 16 + e * 2 + q;
+                in = b == nf && kk < tl;
+                if (in) val = __bfloat162float(vt[dim * 32 + kk]);
+              } else {
+                in = b == nf && key % 32 < tl;
+                if (in) val = __bfloat162float(kt[((rw / BN) * 32 + key % 32) * 64 + el]);
+              }
+              f[q] = in ? val * up : 0.f;
+            }
+            const uint32_t z = pack_f16x2(f[0], f[1]);
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (q == e) y[q] = z;
+          }
+        }
+        unsigned char* p = reinterpret_cast<unsigned char*>(dst) + rw * 128;
+        *reinterpret_cast<uint4*>(p + (((2 * part) ^ (rw & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(p + (((2 * part + 1) ^ (rw & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+      }
+    };
+    if (nb > 0) load(jb, false, xk);
+    for (int i = 0; i < nb; ++i) {
+      const int j = jb + i, st = i & 1;
+      load(j, true, xv);
+      if (i >= 2) ok = tc::mbar_wait(&s->k_empty[st], ((i >> 1) - 1) & 1, a.err, 7001);
+      if (!__all_sync(0xffffffffu, ok) || *(volatile int*)&s->abort) break;
+      store(j, false, xk, s->K[st]);
+      if (tid < NG) {
+        const int b = j * NG + tid;
+        const float k1 = b < nf ? ks[b] : b == nf && tl ? s->tail[1] : 0.f;
+        const float v1 = b < nf ? vs[b] : b == nf && tl ? s->tail[3] : 0.f;
+        s->kmul[i & 3][tid] = k1 > 0.f ? k1 : 1.f;  // a block of zeros: any factor
+        s->vadd[i & 3][tid] = v1 > 0.f ? log2f(v1 / vref) : 0.f;
+        s->vinv[i & 3][tid] = v1 > 0.f ? vref / v1 : 1.f;
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&s->k_full[st]);
+      if (tid == 0) tc::mbar_arrive(&s->sc_full[i & 3]);
+      if (i + 1 < nb) load(j + 1, false, xk);
+      if (i >= 2) ok = tc::mbar_wait(&s->v_empty[st], ((i >> 1) - 1) & 1, a.err, 7002);
+      if (!__all_sync(0xffffffffu, ok) || *(volatile int*)&s->abort) break;
+      store(j, true, xv, s->V[st]);
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&s->v_full[st]);
+    }
+    if (!ok) s->abort = 1;
+  } else if (warp == MMA_WARP) {
+    // ------------------------------------ MMA issuer ---------------------------------------------
+    if (lane == 0 && nb > 0) {
+      constexpr uint32_t id_s = idesc_f16_f32(128, BN), id_o = idesc_f16_f32(128, D);
+      const int items = nb * NT;  // item i: tile i % NT, key tile i / NT, score buffer i % 2
+      bool ok = tc::mbar_wait(&s->q_full, 0, a.err, 7003);
+      auto qk = [&](int i) {
+        const int j = i / NT, u = i % NT, st = j & 1;
+        if (u == 0 && !tc::mbar_wait(&s->k_full[st], (j >> 1) & 1, a.err, 7004)) return false;
+        tc::tc_fence_after();
+        const uint32_t q0 = tc::smem_u32(s->Q[u]), k0 = tc::smem_u32(s->K[st]);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16_ss(tmem + S_COL + (i & 1) * BN, tc::sdesc_k128(q0 + (k >> 2) * 128 * 128 + (k & 3) * 32),
+                      tc::sdesc_k128(k0 + (k >> 2) * BN * 128 + (k & 3) * 32), id_s, k > 0);
+        tc::umma_commit(&s->s_full[i & 1]);
+        if (u == NT - 1) tc::umma_commit(&s->k_empty[st]);
+        return true;
+      };
+      auto pv = [&](int i) {
+        const int j = i / NT, u = i % NT, st = j & 1;
+        if (u == 0 && !tc::mbar_wait(&s->v_full[st], (j >> 1) & 1, a.err, 7005)) return false;
+        if (!tc::mbar_wait(&s->p_full[i & 1], (i >> 1) & 1, a.err, 7006)) return false;
+        tc::tc_fence_after();
+        const uint32_t v0 = tc::smem_u32(s->V[st]);
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)
+          umma_f16_ts(tmem + u * D, tmem + S_COL + (i & 1) * BN + k * 8,
+                      tc::sdesc_k128(v0 + (k >> 2) * D * 128 + (k & 3) * 32), id_o, (j > 0 || k > 0) ? 1u : 0u);
+        tc::umma_commit(&s->o_done[u]);
+        if (u == NT - 1) tc::umma_commit(&s->v_empty[st]);
+        return true;
+      };
+      ok = ok && qk(0);
+      for (int i = 0; i < items && ok && !*(volatile int*)&s->abort; ++i) {
+        // the scores of item i + 1 go where P of item i - 1 was: that product is ahead in the pipe
+        if (i + 1 < items) ok = qk(i + 1);
+        ok = ok && pv(i);
+      }
+      if (!ok) s->abort = 1;
+    }
+  } else {
+    // ------------------------------------ softmax ------------------------------------------------
+    const int q = warp & 3;              // TMEM lane quarter of this warp
+    const int u = (warp - 4) >> 2;       // tile
+    const int row = q * 32 + lane, r = r0 + u * 128 + row;
+    const bool live = r < R;
+    const int t = live ? r / G : a.T - 1, hq = h * G + (live ? r % G : 0), pos = a.p0 + t;
+    const uint32_t lane_at = (uint32_t)(q * 32) << 16;
+    float qs;  // score factor of the row
+    {
+      const __nv_bfloat16* src = a.q + t * a.ldq + (long long)hq * D;
+      float mag = 0.f;
+      float f[16];
+#pragma unroll 1
+      for (int d = 0; d < D; d += 16) {
+        load16(src, d, a.vec_q, f);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mag = fmaxf(mag, kv8_mag(f[e]));
+      }
+      float up, down;
+      pow2_scale(mag, &up, &down);
+      qs = a.sl2 * down;
+      unsigned char* base = reinterpret_cast<unsigned char*>(s->Q[u]) + row * 128;
+#pragma unroll 1
+      for (int d = 0; d < D; d += 16) {
+        load16(src, d, a.vec_q, f);
+        uint32_t y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = live ? pack_f16x2(f[2 * e] * up, f[2 * e + 1] * up) : 0u;
+        unsigned char* p = base + (d >> 6) * (128 * 128);
+        const int un = (d & 63) >> 3;
+        *reinterpret_cast<uint4*>(p + ((un ^ (row & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(p + (((un + 1) ^ (row & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&s->q_full);
+    }
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    // tcgen05.ld / st run with the whole warp: every branch around them is warp-uniform
+    for (int j = 0; j < nb; ++j) {
+      const int i = j * NT + u, sl = i & 1;
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(&s->s_full[sl], (i >> 1) & 1, a.err, 7007))) { ok = false; break; }
+      // The tile's scale factors. Tile j + 4 overwrites them after P_j was consumed, so this wait
+      // is never more than one phase behind (k_full, refilled after Q K_j, could be two).
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(&s->sc_full[j & 3], (j >> 2) & 1, a.err, 7008))) { ok = false; break; }
+      tc::tc_fence_after();
+      const uint32_t sa = tmem + lane_at + S_COL + sl * BN;
+      const int k0 = (jb + j) * BN;
+      const bool diag = k0 + BN > a.p0 + (r0 + u * 128) / G + 1;  // some row of the tile may end inside
+      const int lim = pos + 1 - k0;                               // keys of this tile that the row sees
+      float km[NG];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) km[g] = s->kmul[j & 3][g] * qs;
+#pragma unroll
+      for (int c = 0; c < BN / 64; ++c) {
+        float x[64];
+        tmem_ld64(sa + c * 64, x);
+        if (diag)
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (c * 64 + e >= lim) x[e] = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float y = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) y = fmaxf(y, x[g * 32 + e]);
+          mx = fmaxf(mx, y * km[c * 2 + g]);
+        }
+      }
+      const bool grow = mx > m + 8.f;  // the row's max moved past the lazy bound
+      const bool mine = grow && l > 0.f;
+      float f = 1.f;
+      if (mine) {
+        f = exp2_fast(m - mx);
+        l *= f;
+      }
+      if (grow) m = mx;
+      if (__any_sync(0xffffffffu, mine)) {  // O (this tile's products so far) to the new max
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(&s->o_done[u], (j - 1) & 1, a.err, 7009))) { ok = false; break; }
+        tc::tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          tc::tmem_ld32(tmem + lane_at + u * D + c * 32, o);
+          uint32_t y[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(o[e] * f);
+          tmem_st32(tmem + lane_at + u * D + c * 32, y);
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m - 6.f;  // P up to 2^6, and 2^14 before a rescale
+#pragma unroll
+      for (int c = 0; c < BN / 64; ++c) {
+        float x[64];
+        tmem_ld64(sa + c * 64, x);
+        if (diag)
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (c * 64 + e >= lim) x[e] = -INFINITY;
+        uint32_t y[32];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const float b = s->vadd[j & 3][c * 2 + g] - base;
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float p0 = exp2_fast(fmaf(x[g * 32 + e], km[c * 2 + g], b));
+            const float p1 = exp2_fast(fmaf(x[g * 32 + e + 1], km[c * 2 + g], b));
+            sum += p0 + p1;
+            y[g * 16 + e / 2] = pack_f16x2(p0, p1);
+          }
+          l = fmaf(sum, s->vinv[j & 3][c * 2 + g], l);
+        }
+        tmem_st32(sa + c * 32, y);  // over scores that this thread has read twice
+      }
+      tmem_wait_st();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&s->p_full[sl]);
+    }
+    // ---- epilogue ----------------------------------------------------------------------------------
+    if (nb > 0) {
+      if (ok && __all_sync(0xffffffffu, tc::mbar_wait(&s->o_done[u], (nb - 1) & 1, a.err, 7010))) {
+        tc::tc_fence_after();
+        const float inv = l > 0.f ? vref / l : 0.f;
+        const bool split = gridDim.z > 1;
+        const long long pr = ((long long)blockIdx.z * a.c.Hkv + h) * R + r;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          tc::tmem_ld32(tmem + lane_at + u * D + c * 32, o);
+          if (!live) continue;
+          if (split) {
+            float4* dst = reinterpret_cast<float4*>(a.part + pr * D + c * 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              dst[e] = make_float4(o[4 * e] * vref, o[4 * e + 1] * vref, o[4 * e + 2] * vref, o[4 * e + 3] * vref);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= inv;
+            finish16(a, t, hq, c * 32, o);
+            finish16(a, t, hq, c * 32 + 16, o + 16);
+          }
+        }
+        if (split && live) reinterpret_cast<float2*>(a.part_ml)[pr] = make_float2(m, l);
+      } else {
+        ok = false;
+      }
+    } else if (live && gridDim.z > 1) {
+      reinterpret_cast<float2*>(a.part_ml)[((long long)blockIdx.z * a.c.Hkv + h) * R + r] = make_float2(-INFINITY, 0.f);
+    }
+    if (!ok) s->abort = 1;
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// One warp a row: the splits' partials, each relative to its own max, to the output.
+template <int D>
+__global__ void __launch_bounds__(128) attn_prefill_kv8_merge(AttnPrefillKV8Args a) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, G = a.Hq / a.c.Hkv, R = a.T * G;
+  const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (i >= (long long)a.c.Hkv * R) return;
+  const int h = (int)(i / R), r = (int)(i % R);
+  const long long stride = (long long)a.c.Hkv * R;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < a.splits) ml = reinterpret_cast<const float2*>(a.part_ml)[lane * stride + i];
+  const float M = warp_max(ml.x);
+  const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - M);
+  const float l = warp_sum(ml.y * f), w = l > 0.f ? f / l : 0.f;
+  constexpr int PER = D / 32;
+  float o[PER] = {};
+#pragma unroll 4
+  for (int z = 0; z < a.splits; ++z) {
+    const float wz = __shfl_sync(0xffffffffu, w, z);
+    if (wz == 0.f) continue;  // a split without keys wrote nothing
+    const float* p = a.part + (z * stride + i) * D;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] = fmaf(p[e * 32 + lane], wz, o[e]);
+  }
+  const int t = r / G, hq = h * G + r % G;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const int d = e * 32 + lane;
+    float x = o[e];
+    if (a.gate) x = __fdividef(x, 1.f + __expf(-__bfloat162float(a.gate[t * a.ldg_t + hq * a.ldg_h + d])));
+    a.o[t * a.ldo + (long long)hq * D + d] = __float2bfloat16(x);
+  }
+}
+
+template <int D, int NT, int BN, bool FP8>
+static cudaError_t launch_prefill(const AttnPrefillKV8Args& a, cudaStream_t st) {
+  auto k = attn_prefill_kv8_kernel<D, NT, BN, FP8>;
+  const size_t smem = sizeof(PrefillKV8Smem<D, NT, BN>) + 1024;
+  static_assert(sizeof(PrefillKV8Smem<D, NT, BN>) + 1024 <= 227 * 1024, "shared memory");
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const int R = a.T * (a.Hq / a.c.Hkv);
+  e = hx_launch_pdl(k, dim3((unsigned)a.c.Hkv, (unsigned)((R + 128 * NT - 1) / (128 * NT)), (unsigned)a.splits),
+                    dim3(160 + 128 * NT), smem, st, a);
+  if (e != cudaSuccess || a.splits == 1) return e;
+  return hx_launch_pdl(attn_prefill_kv8_merge<D>, dim3((unsigned)(((long long)a.c.Hkv * R + 3) / 4)), dim3(128), 0, st, a);
 }
 
 cudaError_t attn_prefill_kv8_launch(const AttnPrefillKV8Args& a, cudaStream_t st) {
   cudaError_t e = cudaSuccess;
   kv8_dispatch(a.c.D, a.c.fp8, [&](auto d, auto fp8) {
-    constexpr int DD = decltype(d)::value;
-    auto k = attn_prefill_kv8_kernel<DD, decltype(fp8)::value>;
-    const size_t smem = sizeof(KV8RowsSmem<DD>);
-    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = hx_launch_pdl(k, dim3((unsigned)((a.T + kKV8Rows - 1) / kKV8Rows), (unsigned)a.Hq), dim3(128), smem, st, a);
+    constexpr int D = decltype(d)::value;
+    constexpr bool F = decltype(fp8)::value;
+    if constexpr (D == 256) e = launch_prefill<256, 1, 64, F>(a, st);
+    else if (a.NT == 1) e = launch_prefill<D, 1, 128, F>(a, st);
+    else e = launch_prefill<D, 2, 128, F>(a, st);
   });
   return e;
 }

@@ -72,6 +72,18 @@ HX_DEVICE float kv8_inv(float a) { return a < kKV8Least ? 0.f : kv8_top<FP8>() /
 template <bool FP8>
 HX_DEVICE float kv8_scale(float a) { return a < kKV8Least ? 0.f : a / kv8_top<FP8>(); }
 
+// 16 dims from d0 of the row, as floats.
+HX_DEVICE void load16(const __nv_bfloat16* row, int d0, int vec, float* f) {
+  if (vec) {
+    const bf16x8* p = reinterpret_cast<const bf16x8*>(row + d0);
+    unpack8(p[0], f);
+    unpack8(p[1], f + 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = __bfloat162float(row[d0 + i]);
+  }
+}
+
 // Calls f(integral_constant<head dim>, true_type for e4m3 or false_type for int8).
 template <typename F>
 inline void kv8_dispatch(int D, bool fp8, F&& f) {

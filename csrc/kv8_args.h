@@ -82,6 +82,11 @@ struct AttnPrefillKV8Args {
   __nv_bfloat16* o;
   long long ldq, ldo, ldg_t, ldg_h;
   int slot, T, p0, Hq;
+  int vec_q, vec_o, vec_g;    // rows of q, o, gate are 16-byte aligned
+  int NT, splits;             // row tiles of a CTA; CTAs that share a row's keys
+  float* part;                // [splits, Hkv, T * G, D] where splits > 1
+  float* part_ml;             // [splits, Hkv, T * G, 2]
+  int* err;
   float sl2;
 };
 cudaError_t attn_prefill_kv8_launch(const AttnPrefillKV8Args& a, cudaStream_t st);

@@ -12,18 +12,6 @@
 
 namespace hx {
 
-// 16 dims from d0 of the row, as floats.
-HX_DEVICE void load16(const __nv_bfloat16* row, int d0, int vec, float* f) {
-  if (vec) {
-    const bf16x8* p = reinterpret_cast<const bf16x8*>(row + d0);
-    unpack8(p[0], f);
-    unpack8(p[1], f + 8);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = __bfloat162float(row[d0 + i]);
-  }
-}
-
 // One block of one head: grid (blocks, Hkv, 2), z = 0 for K and 1 for V. Piece i of a thread
 // is 16 dims of one key: for K, four neighbouring lanes hold the 64 dims of a panel's row;
 // for V, a warp holds the same dims of the 32 keys, so that their codes, written to shared

@@ -240,5 +240,25 @@ void attn_prefill_kv8(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torch
   a.ldo = out.stride(0);
   a.slot = (int)slot; a.T = (int)T; a.p0 = (int)p0; a.Hq = (int)Hq;
   a.sl2 = (float)scale * 1.4426950408889634f;
+  auto aligned = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; };
+  a.vec_q = aligned(a.q, T > 1 ? a.ldq : 0);
+  a.vec_o = aligned(a.o, T > 1 ? a.ldo : 0);
+  a.vec_g = gate && aligned(a.gate, T > 1 ? a.ldg_t : 0) && a.ldg_h % 8 == 0;
+  a.err = err.data_ptr<int>();
+  // Two row tiles a CTA where there are rows for them (at head dim 256 TMEM holds one), and CTAs
+  // for every SM: with fewer the keys are split, at least four key tiles to a part.
+  const int64_t R = T * (Hq / Hkv);
+  TORCH_CHECK(R < (1ll << 31), "T * query heads of a kv head past 2^31");
+  a.NT = D <= 128 && R > 128 ? 2 : 1;
+  const int64_t ctas = (R + 128 * a.NT - 1) / (128 * a.NT) * Hkv;
+  const int sms = at::cuda::getDeviceProperties(kc.device().index())->multiProcessorCount;
+  const int64_t tiles = (p0 + T + 127) / 128;
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / ctas, tiles / 4, 32}));
+  torch::Tensor part;
+  if (a.splits > 1) {
+    part = torch::empty({a.splits * Hkv * R * (D + 2)}, ks.options());
+    a.part = part.data_ptr<float>();
+    a.part_ml = a.part + a.splits * Hkv * R * D;
+  }
   HX_KV8_LAUNCH(attn_prefill_kv8_launch(a, at::cuda::getCurrentCUDAStream()));
 }
