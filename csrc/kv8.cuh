@@ -62,26 +62,72 @@ HX_DEVICE float kv8_float(uint8_t c) {
   else return (float)(int8_t)c;
 }
 
-// |x| for the block maximum: infinities and NaN do not count.
+// The same for finite values, |x * inv| <= M: int8 codes are the low bytes after adding 1.5 * 2^23,
+// which rounds to whole numbers, ties to even (no conversion instruction: those issue at an eighth
+// of the rate).
+template <bool FP8>
+HX_DEVICE uint32_t kv8_code4_finite(const float* x, float inv) {
+  if constexpr (FP8) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inv, x[1] * inv), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inv, x[3] * inv), __NV_SATFINITE, __NV_E4M3);
+    return lo | hi << 16;
+  } else {
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.f));
+    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+  }
+}
+
+// |x| where infinities and NaN do not count.
 HX_DEVICE float kv8_mag(float x) {
   const float a = fabsf(x);
   return a <= 3.4028235e38f ? a : 0.f;
 }
+
+// Block maxima of packed bf16 pairs: |x| grows with the bits without the sign; from kKV8Inf on they
+// are infinities and NaN, and the pairs are taken again without those.
+constexpr uint32_t kKV8Inf = 0x7f80u;
+HX_DEVICE uint32_t kv8_max2(uint32_t m, uint32_t x) { return __vmaxu2(m, x & 0x7fff7fffu); }
+HX_DEVICE uint32_t kv8_max2_finite(uint32_t m, uint32_t x) {
+  const uint32_t lo = x & 0x7fffu, hi = x >> 16 & 0x7fffu;
+  return __vmaxu2(m, (lo < kKV8Inf ? lo : 0u) | (hi < kKV8Inf ? hi : 0u) << 16);
+}
+HX_DEVICE uint32_t kv8_max1(uint32_t m) { return __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16)); }
+HX_DEVICE float kv8_bits(uint32_t m) { return __uint_as_float(m << 16); }
+
+// Codes of eight packed bf16 values.
+template <bool FP8>
+HX_DEVICE uint2 kv8_code8(const uint4& x, float inv, bool special) {
+  float f[8];
+  unpack8(*reinterpret_cast<const bf16x8*>(&x), f);
+  if (special) return make_uint2(kv8_code4<FP8>(f, inv), kv8_code4<FP8>(f + 4, inv));
+  return make_uint2(kv8_code4_finite<FP8>(f, inv), kv8_code4_finite<FP8>(f + 4, inv));
+}
+
 template <bool FP8>
 HX_DEVICE float kv8_inv(float a) { return a < kKV8Least ? 0.f : kv8_top<FP8>() / a; }
 template <bool FP8>
 HX_DEVICE float kv8_scale(float a) { return a < kKV8Least ? 0.f : a / kv8_top<FP8>(); }
 
-// 16 dims from d0 of the row, as floats.
-HX_DEVICE void load16(const __nv_bfloat16* row, int d0, int vec, float* f) {
+// 8 dims from d0 of a row as they are, and 8 or 16 as floats.
+HX_DEVICE uint4 load8_raw(const __nv_bfloat16* row, int d0, int vec) {
+  if (vec) return *reinterpret_cast<const uint4*>(row + d0);
+  const unsigned short* p = reinterpret_cast<const unsigned short*>(row + d0);
+  return make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16,
+                    p[6] | (uint32_t)p[7] << 16);
+}
+HX_DEVICE void load8(const __nv_bfloat16* row, int d0, int vec, float* f) {
   if (vec) {
-    const bf16x8* p = reinterpret_cast<const bf16x8*>(row + d0);
-    unpack8(p[0], f);
-    unpack8(p[1], f + 8);
+    unpack8(*reinterpret_cast<const bf16x8*>(row + d0), f);
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = __bfloat162float(row[d0 + i]);
+    for (int i = 0; i < 8; ++i) f[i] = __bfloat162float(row[d0 + i]);
   }
+}
+HX_DEVICE void load16(const __nv_bfloat16* row, int d0, int vec, float* f) {
+  load8(row, d0, vec, f);
+  load8(row, d0 + 8, vec, f + 8);
 }
 
 // Calls f(integral_constant<head dim>, true_type for e4m3 or false_type for int8).

@@ -9,76 +9,119 @@
 // threads takes one block of one kv head, of K or of V, and keeps it in registers between the
 // maximum and the codes, so each value is read once.
 #include "kv8.cuh"
+#include "kv8_f16.cuh"
 
 namespace hx {
 
-// One block of one head: grid (blocks, Hkv, 2), z = 0 for K and 1 for V. Piece i of a thread
-// is 16 dims of one key: for K, four neighbouring lanes hold the 64 dims of a panel's row;
-// for V, a warp holds the same dims of the 32 keys, so that their codes, written to shared
-// memory a byte each, become rows of 32 keys.
+// Byte b of word r of the answer is byte r of word b.
+HX_DEVICE void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t* w) {
+  const uint32_t p = __byte_perm(a, b, 0x5140), q = __byte_perm(a, b, 0x7362);
+  const uint32_t r = __byte_perm(c, d, 0x5140), s = __byte_perm(c, d, 0x7362);
+  w[0] = __byte_perm(p, r, 0x5410);
+  w[1] = __byte_perm(p, r, 0x7632);
+  w[2] = __byte_perm(q, s, 0x5410);
+  w[3] = __byte_perm(q, s, 0x7632);
+}
+
+// One block of one head: grid (blocks, Hkv, 2), z = 0 for K and 1 for V. A thread's piece of K
+// is 16 dims of one key (four lanes hold a panel's row); of V 8 dims of 4 keys, whose codes are
+// words of V's rows of 32 keys as they come.
 template <int D, bool FP8>
 __global__ void __launch_bounds__(128) kv8_append_kernel(KV8AppendArgs a) {
-  constexpr int NP = D / 64;  // pieces of a thread: 32 x D / 16 / 128
-  __shared__ float red[4];
-  __shared__ __align__(16) uint8_t vcode[D * kKV8Block];
+  constexpr int NP = D / 64, NV = (D + 127) / 128;
   pdl_wait_prior();
   pdl_launch_dependents();
   const int b = a.b0 + blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
   const bool isv = blockIdx.z != 0;
   const int L = a.p0 + a.T, j0 = b * kKV8Block;
   const bool whole = j0 + kKV8Block <= L;
-  const long long hd = a.c.head(a.slot, h);
+  const long long hd = a.c.head(a.slot, h), blk = a.c.block(a.slot, h, b);
   const __nv_bfloat16* src = isv ? a.v + h * a.v_head : a.k + h * a.k_head;
   const long long ld = isv ? a.v_row : a.k_row;
   __nv_bfloat16* tail = (isv ? a.c.vt : a.c.kt) + hd * (NP * kKV8Panel);
-  if (whole) {
-    float f[NP][16];
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      // K: 8 keys x 4 pieces of a panel to a warp; V: 32 keys x 1 piece
-      const int key = isv ? (tid & 31) : ((tid >> 5) * 8 + ((tid & 31) >> 2));
-      const int d0 = isv ? (i * 4 + (tid >> 5)) * 16 : i * 64 + (tid & 3) * 16;
-      const int j = j0 + key;
-      if (j >= a.p0) {
-        load16(src + (j - a.p0) * ld, d0, a.vec, f[i]);
-      } else if (!isv) {
-        load16(tail + ((d0 >> 6) * kKV8Block + key) * 64 + (d0 & 63), 0, 1, f[i]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) f[i][e] = __bfloat162float(tail[(d0 + e) * kKV8Block + key]);
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) m = fmaxf(m, kv8_mag(f[i][e]));
-    }
-    m = warp_max(m);
-    if ((tid & 31) == 0) red[tid >> 5] = m;
+  __shared__ uint32_t redu[2][4];
+  // maximum over the CTA's packed pairs; `round` 0, then 1 if the block holds an infinity or a NaN
+  auto block_max = [&](uint32_t m, int round) {
+    m = kv8_max1(m);
+    if ((tid & 31) == 0) redu[round][tid >> 5] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float inv = kv8_inv<FP8>(m);
-    uint8_t* dst = (isv ? a.c.vc : a.c.kc) + a.c.block(a.slot, h, b) * (NP * kKV8Panel);
-    if (tid == 0) (isv ? a.c.vs : a.c.ks)[a.c.block(a.slot, h, b)] = kv8_scale<FP8>(m);
+    return max(max(redu[round][0], redu[round][1]), max(redu[round][2], redu[round][3]));
+  };
+  // K: two halves of 16 dims of a key; V: 8 dims of each of four keys
+  constexpr int NX = NP > 2 * NV ? NP : 2 * NV;
+  uint4 x[NX][2];
+  const int key = tid >> 2, part = (tid & 3) * 16, q = tid & 7, dq = (tid >> 3) * 8;
+  if (whole) {
+    uint32_t m = 0;
+    auto pass = [&](auto&& f) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
+      for (int i = 0; i < NX; ++i)
+        if (isv ? (i >> 1) * 128 + dq < D && i < 2 * NV : i < NP) f(i);
+    };
+    pass([&](int i) {
       if (!isv) {
-        const int key = (tid >> 5) * 8 + ((tid & 31) >> 2);
-        *reinterpret_cast<uint4*>(dst + (i * kKV8Block + key) * 64 + (tid & 3) * 16) =
-            make_uint4(kv8_code4<FP8>(f[i], inv), kv8_code4<FP8>(f[i] + 4, inv), kv8_code4<FP8>(f[i] + 8, inv),
-                       kv8_code4<FP8>(f[i] + 12, inv));
+        const int j = j0 + key;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          x[i][e] = j >= a.p0 ? load8_raw(src + (j - a.p0) * ld, i * 64 + part + e * 8, a.vec)
+                              : load8_raw(tail + (i * kKV8Block + key) * 64, part + e * 8, 1);
       } else {
-        const int d0 = (i * 4 + (tid >> 5)) * 16;
+        const int d0 = (i >> 1) * 128 + dq;
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const uint32_t q = kv8_code4<FP8>(f[i] + e, inv);
+        for (int e = 0; e < 2; ++e) {
+          const int k = (i & 1) * 2 + e, j = j0 + 4 * q + k;
+          if (j >= a.p0) {
+            x[i][e] = load8_raw(src + (j - a.p0) * ld, d0, a.vec);
+          } else {
+            uint32_t y[8];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) vcode[(d0 + e + c) * kKV8Block + (tid & 31)] = (uint8_t)(q >> 8 * c);
+            for (int c = 0; c < 8; ++c) y[c] = __bfloat16_as_ushort(tail[(d0 + c) * kKV8Block + 4 * q + k]);
+            x[i][e] = make_uint4(y[0] | y[1] << 16, y[2] | y[3] << 16, y[4] | y[5] << 16, y[6] | y[7] << 16);
+          }
         }
       }
+    });
+    pass([&](int i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        m = kv8_max2(kv8_max2(kv8_max2(kv8_max2(m, x[i][e].x), x[i][e].y), x[i][e].z), x[i][e].w);
+    });
+    m = block_max(m, 0);
+    const bool special = m >= kKV8Inf;
+    if (special) {
+      m = 0;
+      pass([&](int i) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          m = kv8_max2_finite(kv8_max2_finite(kv8_max2_finite(kv8_max2_finite(m, x[i][e].x), x[i][e].y), x[i][e].z), x[i][e].w);
+      });
+      m = block_max(m, 1);
     }
-    __syncthreads();
-    if (isv)
-      for (int i = tid; i < D * kKV8Block / 16; i += 128)
-        reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(vcode)[i];
+    if (tid == 0) (isv ? a.c.vs : a.c.ks)[blk] = kv8_scale<FP8>(kv8_bits(m));
+    const float inv = kv8_inv<FP8>(kv8_bits(m));
+    if (!isv) {
+      uint8_t* dst = a.c.kc + blk * (NP * kKV8Panel);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const uint2 u = kv8_code8<FP8>(x[i][0], inv, special), w = kv8_code8<FP8>(x[i][1], inv, special);
+        *reinterpret_cast<uint4*>(dst + (i * kKV8Block + key) * 64 + part) = make_uint4(u.x, u.y, w.x, w.y);
+      }
+    } else {
+      uint8_t* dst = a.c.vc + blk * (NP * kKV8Panel);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int d0 = i * 128 + dq;
+        if (d0 >= D) continue;
+        uint2 c[4];  // eight dims' codes of each key
+#pragma unroll
+        for (int k = 0; k < 4; ++k) c[k] = kv8_code8<FP8>(x[2 * i + (k >> 1)][k & 1], inv, special);
+        uint32_t w[8];
+        transpose4(c[0].x, c[1].x, c[2].x, c[3].x, w);
+        transpose4(c[0].y, c[1].y, c[2].y, c[3].y, w + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) *reinterpret_cast<uint32_t*>(dst + (d0 + e) * kKV8Block + 4 * q) = w[e];
+      }
+    }
   }
   // The first block's CTA alone has read the old tail (above), so it writes the new one: the
   // new rows of the sequence's last block.
@@ -102,11 +145,25 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(KV8AppendArgs a) {
   }
 }
 
-// Grid (blocks, Hkv, 2) of 128 threads as in the append; a thread writes 32 bytes of a row.
+// Four codes times the scale, each rounded once to bf16.
+template <bool FP8>
+HX_DEVICE uint2 codes_to_bf16(uint32_t w, float scale) {
+  uint32_t lo, hi;
+  codes_to_f16<FP8>(w, lo, hi);
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+  const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  const __nv_bfloat162 p = __floats2bfloat162_rn(x.x * scale, x.y * scale);
+  const __nv_bfloat162 q = __floats2bfloat162_rn(y.x * scale, y.y * scale);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&p), *reinterpret_cast<const uint32_t*>(&q));
+}
+
+// Grid (blocks, Hkv, 2) of 128 threads. K: a thread's pieces are as in the append. V: the block's
+// codes go through shared memory (rows of 36 bytes: the words that a warp reads lie in different
+// banks); a thread takes words of 4 keys from 8 dims' rows and turns them into 8 dims of 4 keys.
 template <int D, bool FP8>
 __global__ void __launch_bounds__(128) kv8_read_kernel(KV8ReadArgs a) {
-  constexpr int NP = D / 64;
-  __shared__ __align__(16) uint8_t vcode[D * kKV8Block];
+  constexpr int NP = D / 64, NV = (D + 127) / 128, LDV = 9;
+  __shared__ uint32_t vcode[D * LDV];
   pdl_wait_prior();
   pdl_launch_dependents();
   const int b = a.start / kKV8Block + blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
@@ -114,42 +171,62 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(KV8ReadArgs a) {
   const int j0 = b * kKV8Block;
   const bool whole = j0 + kKV8Block <= a.L;
   const long long blk = a.c.block(a.slot, h, b);
-  const uint8_t* codes = (isv ? a.c.vc : a.c.kc) + blk * (NP * kKV8Panel);
-  const __nv_bfloat16* tail = (isv ? a.c.vt : a.c.kt) + a.c.head(a.slot, h) * (NP * kKV8Panel);
-  const float scale = whole ? (isv ? a.c.vs : a.c.ks)[blk] : 0.f;
-  if (isv && whole) {
-    for (int i = tid; i < D * kKV8Block / 16; i += 128)
-      reinterpret_cast<uint4*>(vcode)[i] = reinterpret_cast<const uint4*>(codes)[i];
-    __syncthreads();
-  }
   __nv_bfloat16* out = isv ? a.v + h * a.v_head : a.k + h * a.k_head;
   const long long ld = isv ? a.v_row : a.k_row;
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int key = isv ? (tid & 31) : ((tid >> 5) * 8 + ((tid & 31) >> 2));
-    const int d0 = isv ? (i * 4 + (tid >> 5)) * 16 : i * 64 + (tid & 3) * 16;
-    const int j = j0 + key;
-    if (j < a.start || j >= a.start + a.n) continue;
-    float f[16];
-    if (!whole) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int d = d0 + e;
-        f[e] = __bfloat162float(isv ? tail[d * kKV8Block + key]
-                                    : tail[((d >> 6) * kKV8Block + key) * 64 + (d & 63)]);
-      }
-    } else if (isv) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) f[e] = kv8_float<FP8>(vcode[(d0 + e) * kKV8Block + key]) * scale;
-    } else {
-      const uint4 w = *reinterpret_cast<const uint4*>(codes + (i * kKV8Block + key) * 64 + (tid & 3) * 16);
-      const uint8_t* q = reinterpret_cast<const uint8_t*>(&w);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) f[e] = kv8_float<FP8>(q[e]) * scale;
+  auto in = [&](int j) { return j >= a.start && j < a.start + a.n; };
+  if (!whole) {
+    const __nv_bfloat16* tail = (isv ? a.c.vt : a.c.kt) + a.c.head(a.slot, h) * (NP * kKV8Panel);
+    for (int i = tid; i < kKV8Block * D; i += 128) {
+      const int key = i / D, d = i % D, j = j0 + key;
+      if (in(j))
+        out[(long long)(j - a.start) * ld + d] =
+            isv ? tail[d * kKV8Block + key] : tail[((d >> 6) * kKV8Block + key) * 64 + (d & 63)];
     }
-    bf16x8* p = reinterpret_cast<bf16x8*>(out + (long long)(j - a.start) * ld + d0);
-    p[0] = pack8(f);
-    p[1] = pack8(f + 8);
+  } else if (!isv) {
+    const uint8_t* codes = a.c.kc + blk * (NP * kKV8Panel);
+    const float scale = a.c.ks[blk];
+    const int key = tid >> 2, part = (tid & 3) * 16, j = j0 + key;
+    uint4 w[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) w[i] = ld_stream_u4(reinterpret_cast<const uint4*>(codes + (i * kKV8Block + key) * 64 + part));
+    if (in(j))
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const uint2 x = codes_to_bf16<FP8>(w[i].x, scale), y = codes_to_bf16<FP8>(w[i].y, scale);
+        const uint2 z = codes_to_bf16<FP8>(w[i].z, scale), u = codes_to_bf16<FP8>(w[i].w, scale);
+        uint4* p = reinterpret_cast<uint4*>(out + (long long)(j - a.start) * ld + i * 64 + part);
+        p[0] = make_uint4(x.x, x.y, y.x, y.y);
+        p[1] = make_uint4(z.x, z.y, u.x, u.y);
+      }
+  } else {
+    const uint4* codes = reinterpret_cast<const uint4*>(a.c.vc + blk * (NP * kKV8Panel));
+    const float scale = a.c.vs[blk];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = i * 128 + tid;
+      const uint4 w = ld_stream_u4(codes + c);
+      uint32_t* p = vcode + (c >> 1) * LDV + (c & 1) * 4;
+      p[0] = w.x; p[1] = w.y; p[2] = w.z; p[3] = w.w;
+    }
+    __syncthreads();
+    const int q = tid & 7;  // keys 4 q .. 4 q + 3
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int d0 = (i * 16 + (tid >> 3)) * 8;
+      if (d0 >= D) continue;
+      uint32_t w[8], t[2][4];  // t: codes of 4 dims of each key
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = vcode[(d0 + e) * LDV + q];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) transpose4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3], t[g]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = j0 + 4 * q + k;
+        if (!in(j)) continue;
+        const uint2 x = codes_to_bf16<FP8>(t[0][k], scale), y = codes_to_bf16<FP8>(t[1][k], scale);
+        *reinterpret_cast<uint4*>(out + (long long)(j - a.start) * ld + d0) = make_uint4(x.x, x.y, y.x, y.y);
+      }
+    }
   }
 }
 
