@@ -208,69 +208,78 @@ __global__ void __launch_bounds__(160 + 128 * NT, 1) attn_prefill_kv8_kernel(Att
     // ------------------------------------ converters ---------------------------------------------
     // A piece is 16 codes (32 bytes of f16): for K 16 dims of a key, for V 16 keys of a dim. Four
     // neighbouring lanes hold one 128-byte row of a chunk, so stores meet no bank twice.
-    constexpr int PC = BN * D / 16 / 128;  // pieces of a thread
-    const int row8 = lane >> 2, part = lane & 3;
+    constexpr int PC = BN * D / 16 / 128;  // pieces of a thread: step i is 32 rows of the tile's chunks
+    const int r8 = warp * 8 + (lane >> 2), part = lane & 3;  // row in the step; 16 values of it
     bool ok = true;
     uint4 xk[PC], xv[PC];
-    // piece i: eight rows (warp + 4 i) * 8 .. + 7 of the tile's chunks
-    auto load = [&](int j, bool isv, uint4 (&x)[PC]) {
+    // rows of K: (chunk of dims, key), 32 keys are a block's panel; of V: (chunk of two blocks, dim)
+    const uint8_t* kp = kc + r8 * 64 + part * 16;
+    const uint8_t* vp = vc + (part >> 1) * (D * kKV8Block) + r8 * kKV8Block + (part & 1) * 16;
+    const int w0 = r8 * 128 + (((2 * part) ^ (r8 & 7)) << 4), w1 = r8 * 128 + (((2 * part + 1) ^ (r8 & 7)) << 4);
+    auto whole = [&](int j) { return (j + 1) * NG <= nf; };
+    auto load_k = [&](int j) {
+      if (!whole(j)) return;
+      const uint8_t* p = kp + (long long)j * (NG * D * kKV8Block);
 #pragma unroll
-      for (int i = 0; i < PC; ++i) {
-        const int rw = (warp + 4 * i) * 8 + row8;        // row over all chunks
-        if (!isv) {
-          const int c = rw / BN, key = rw % BN, b = j * NG + key / 32;
-          if (b < nf) x[i] = __ldg(reinterpret_cast<const uint4*>(kc + ((long long)b * NP + c) * kKV8Panel + (key % 32) * 64 + part * 16));
-        } else {
-          const int c = rw / D, dim = rw % D, b = j * NG + c * 2 + (part >> 1);
-          if (b < nf) x[i] = __ldg(reinterpret_cast<const uint4*>(vc + (long long)b * (D * kKV8Block) + dim * 32 + (part & 1) * 16));
-        }
-      }
+      for (int i = 0; i < PC; ++i) xk[i] = ld_stream_u4(reinterpret_cast<const uint4*>(p + ((i % NG) * NP + i / NG) * kKV8Panel));
     };
-    auto store = [&](int j, bool isv, const uint4 (&x)[PC], __half* dst) {
+    auto load_v = [&](int j) {
+      if (!whole(j)) return;
+      const uint8_t* p = vp + (long long)j * (NG * D * kKV8Block);
 #pragma unroll
-      for (int i = 0; i < PC; ++i) {
-        const int rw = (warp + 4 * i) * 8 + row8;
-        const int key = isv ? 0 : rw % BN, c = isv ? rw / D : 0, dim = isv ? rw % D : 0;
-        const int b = isv ? j * NG + c * 2 + (part >> 1) : j * NG + key / 32;
-        uint32_t y[8];
-        if (b < nf) {
-          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) codes_to_f16<FP8>(w[e], y[2 * e], y[2 * e + 1]);
-        } else {  // the tail, or past the sequence: zeros there (their probabilities are zero as well)
-          const float up = s->tail[isv ? 2 : 0];
+      for (int i = 0; i < PC; ++i)
+        xv[i] = ld_stream_u4(reinterpret_cast<const uint4*>(p + (i / (D / 32)) * (2 * D * kKV8Block) + (i % (D / 32)) * (32 * kKV8Block)));
+    };
+    auto put = [&](unsigned char* p, const uint4& x) {
+      uint32_t y[8];
+      codes_to_f16<FP8>(x.x, y[0], y[1]);
+      codes_to_f16<FP8>(x.y, y[2], y[3]);
+      codes_to_f16<FP8>(x.z, y[4], y[5]);
+      codes_to_f16<FP8>(x.w, y[6], y[7]);
+      *reinterpret_cast<uint4*>(p + w0) = make_uint4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint4*>(p + w1) = make_uint4(y[4], y[5], y[6], y[7]);
+    };
+    // a tile with blocks that are not complete: codes, bf16 rows of the tail, zeros past the
+    // sequence (where the probabilities are zero as well)
+    auto put_ragged = [&](int j, bool isv, unsigned char* dst) {
 #pragma unroll 1
-          for (int e = 0; e < 8; ++e) {
-            float f[2];
-            for (int q = 0; q < 2; ++q) {
-              const int el = part * 16 + e * 2 + q;
-              bool in;
-              float val = 0.f;
-              if (isv) {
-                const int kk = (part & 1) * 16 + e * 2 + q;
-                in = b == nf && kk < tl;
-                if (in) val = __bfloat162float(vt[dim * 32 + kk]);
-              } else {
-                in = b == nf && key % 32 < tl;
-                if (in) val = __bfloat162float(kt[((rw / BN) * 32 + key % 32) * 64 + el]);
-              }
-              f[q] = in ? val * up : 0.f;
-            }
-            const uint32_t z = pack_f16x2(f[0], f[1]);
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              if (q == e) y[q] = z;
-          }
+      for (int i = 0; i < PC; ++i) {
+        const int b = j * NG + (isv ? i / (D / 32) * 2 + (part >> 1) : i % NG);
+        const int dim = i % (D / 32) * 32 + r8;  // V
+        unsigned char* p = dst + i * 4096;
+        if (b < nf) {
+          put(p, *reinterpret_cast<const uint4*>(
+                     isv ? vc + (long long)b * (D * kKV8Block) + dim * kKV8Block + (part & 1) * 16
+                         : kc + ((long long)b * NP + i / NG) * kKV8Panel + r8 * 64 + part * 16));
+          continue;
         }
-        unsigned char* p = reinterpret_cast<unsigned char*>(dst) + rw * 128;
-        *reinterpret_cast<uint4*>(p + (((2 * part) ^ (rw & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(p + (((2 * part + 1) ^ (rw & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+        const float up = s->tail[isv ? 2 : 0];
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          float f[2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int key = isv ? (part & 1) * 16 + e * 2 + q : r8;
+            f[q] = b != nf || key >= tl ? 0.f
+                   : up * __bfloat162float(isv ? vt[dim * kKV8Block + key] : kt[(i / NG * kKV8Block + key) * 64 + part * 16 + e * 2 + q]);
+          }
+          *reinterpret_cast<uint32_t*>(p + (e < 4 ? w0 : w1) + (e & 3) * 4) = pack_f16x2(f[0], f[1]);
+        }
       }
     };
-    if (nb > 0) load(jb, false, xk);
+    auto store = [&](int j, bool isv, const uint4 (&x)[PC], __half* tile) {
+      unsigned char* dst = reinterpret_cast<unsigned char*>(tile);
+      if (whole(j)) {
+#pragma unroll
+        for (int i = 0; i < PC; ++i) put(dst + i * 4096, x[i]);
+      } else {
+        put_ragged(j, isv, dst);
+      }
+    };
+    if (nb > 0) load_k(jb);
     for (int i = 0; i < nb; ++i) {
       const int j = jb + i, st = i & 1;
-      load(j, true, xv);
+      load_v(j);
       if (i >= 2) ok = tc::mbar_wait(&s->k_empty[st], ((i >> 1) - 1) & 1, a.err, 7001);
       if (!__all_sync(0xffffffffu, ok) || *(volatile int*)&s->abort) break;
       store(j, false, xk, s->K[st]);
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(160 + 128 * NT, 1) attn_prefill_kv8_kernel(Att
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&s->k_full[st]);
       if (tid == 0) tc::mbar_arrive(&s->sc_full[i & 3]);
-      if (i + 1 < nb) load(j + 1, false, xk);
+      if (i + 1 < nb) load_k(j + 1);
       if (i >= 2) ok = tc::mbar_wait(&s->v_empty[st], ((i >> 1) - 1) & 1, a.err, 7002);
       if (!__all_sync(0xffffffffu, ok) || *(volatile int*)&s->abort) break;
       store(j, true, xv, s->V[st]);
