@@ -12,7 +12,7 @@
 // that takes its largest entry to 128..256. So is every row of q (11 bits stay, entries 2^32
 // below the row's largest vanish).
 //
-//   warps 0-3        converters: 8-bit panels from global memory -> f16 tiles of BN keys in shared
+//   first 4 or 8 warps  converters: 8-bit panels from global memory -> f16 tiles of BN keys in shared
 //                    memory, in the 128-byte-swizzled layout the MMA reads (2-stage rings for K, V);
 //   next 4 NT warps  softmax, a thread a row: scores from TMEM, running max with a lazy rescale of O
 //                    (only when the max grows by more than 2^8), P as f16 back into the score
@@ -111,6 +111,7 @@ HX_DEVICE void finish16(const AttnPrefillKV8Args& a, int t, int hq, int d0, floa
 
 template <int D, int NT, int BN>
 struct PrefillKV8Smem {
+  static constexpr int CW = NT == 1 ? 8 : 4;  // converter warps
   alignas(1024) __half Q[NT][128 * D];  // per tile: D/64 chunks of [128 rows x 64], 128B-swizzled
   alignas(1024) __half K[2][BN * D];    // per stage: D/64 chunks of [BN keys x 64 dims]
   alignas(1024) __half V[2][BN * D];    // per stage: BN/64 chunks of [D dims x 64 keys]
@@ -125,10 +126,10 @@ struct PrefillKV8Smem {
 };
 
 template <int D, int NT, int BN, bool FP8>
-__global__ void __launch_bounds__(160 + 128 * NT, 1) attn_prefill_kv8_kernel(AttnPrefillKV8Args a) {
+__global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 * NT, 1) attn_prefill_kv8_kernel(AttnPrefillKV8Args a) {
   static_assert(NT * D + 2 * BN <= 512, "TMEM: the tiles' O and two score buffers");
   using SM = PrefillKV8Smem<D, NT, BN>;
-  constexpr int NTH = 160 + 128 * NT, MMA_WARP = 4 + 4 * NT, NG = BN / 32, NP = D / 64;
+  constexpr int CW = SM::CW, MMA_WARP = CW + 4 * NT, NTH = 32 * (MMA_WARP + 1), NG = BN / 32, NP = D / 64;
   constexpr uint32_t S_COL = NT * D;
   extern __shared__ __align__(1024) unsigned char raw[];
   SM* s = reinterpret_cast<SM*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -142,9 +143,9 @@ __global__ void __launch_bounds__(160 + 128 * NT, 1) attn_prefill_kv8_kernel(Att
   if (tid == 0) {
     tc::mbar_init(&s->q_full, 4 * NT);
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&s->k_full[i], 4);
+      tc::mbar_init(&s->k_full[i], CW);
       tc::mbar_init(&s->k_empty[i], 1);
-      tc::mbar_init(&s->v_full[i], 4);
+      tc::mbar_init(&s->v_full[i], CW);
       tc::mbar_init(&s->v_empty[i], 1);
       tc::mbar_init(&s->s_full[i], 1);
       tc::mbar_init(&s->p_full[i], 4);
@@ -204,31 +205,33 @@ __global__ void __launch_bounds__(160 + 128 * NT, 1) attn_prefill_kv8_kernel(Att
   __syncthreads();
   const uint32_t tmem = s->tmem_base;
 
-  if (warp < 4) {
+  if (warp < CW) {
     // ------------------------------------ converters ---------------------------------------------
     // A piece is 16 codes (32 bytes of f16): for K 16 dims of a key, for V 16 keys of a dim. Four
     // neighbouring lanes hold one 128-byte row of a chunk, so stores meet no bank twice.
-    constexpr int PC = BN * D / 16 / 128;  // pieces of a thread: step i is 32 rows of the tile's chunks
-    const int r8 = warp * 8 + (lane >> 2), part = lane & 3;  // row in the step; 16 values of it
+    constexpr int PC = BN * D / 16 / (32 * CW);  // pieces of a thread: step i is CW groups of 8 rows
+    constexpr int SR = 8 * CW;                   // rows of a step
+    // row in a step; its row of a 32-row panel and that panel; 16 values of the row
+    const int r0s = warp * 8 + (lane >> 2), r8 = r0s & 31, rp = r0s >> 5, part = lane & 3;
     bool ok = true;
     uint4 xk[PC], xv[PC];
     // rows of K: (chunk of dims, key), 32 keys are a block's panel; of V: (chunk of two blocks, dim)
-    const uint8_t* kp = kc + r8 * 64 + part * 16;
-    const uint8_t* vp = vc + (part >> 1) * (D * kKV8Block) + r8 * kKV8Block + (part & 1) * 16;
-    const int w0 = r8 * 128 + (((2 * part) ^ (r8 & 7)) << 4), w1 = r8 * 128 + (((2 * part + 1) ^ (r8 & 7)) << 4);
+    const uint8_t* kp = kc + rp * (NP * kKV8Panel) + r8 * 64 + part * 16;
+    const uint8_t* vp = vc + (part >> 1) * (D * kKV8Block) + r0s * kKV8Block + (part & 1) * 16;
+    const int w0 = r0s * 128 + (((2 * part) ^ (r8 & 7)) << 4), w1 = r0s * 128 + (((2 * part + 1) ^ (r8 & 7)) << 4);
     auto whole = [&](int j) { return (j + 1) * NG <= nf; };
     auto load_k = [&](int j) {
       if (!whole(j)) return;
       const uint8_t* p = kp + (long long)j * (NG * D * kKV8Block);
 #pragma unroll
-      for (int i = 0; i < PC; ++i) xk[i] = ld_stream_u4(reinterpret_cast<const uint4*>(p + ((i % NG) * NP + i / NG) * kKV8Panel));
+      for (int i = 0; i < PC; ++i) xk[i] = ld_stream_u4(reinterpret_cast<const uint4*>(p + ((i * (SR / 32) % NG) * NP + i * (SR / 32) / NG) * kKV8Panel));
     };
     auto load_v = [&](int j) {
       if (!whole(j)) return;
       const uint8_t* p = vp + (long long)j * (NG * D * kKV8Block);
 #pragma unroll
       for (int i = 0; i < PC; ++i)
-        xv[i] = ld_stream_u4(reinterpret_cast<const uint4*>(p + (i / (D / 32)) * (2 * D * kKV8Block) + (i % (D / 32)) * (32 * kKV8Block)));
+        xv[i] = ld_stream_u4(reinterpret_cast<const uint4*>(p + (i / (D / SR)) * (2 * D * kKV8Block) + (i % (D / SR)) * (SR * kKV8Block)));
     };
     auto put = [&](unsigned char* p, const uint4& x) {
       uint32_t y[8];
@@ -244,13 +247,14 @@ __global__ void __launch_bounds__(160 + 128 * NT, 1) attn_prefill_kv8_kernel(Att
     auto put_ragged = [&](int j, bool isv, unsigned char* dst) {
 #pragma unroll 1
       for (int i = 0; i < PC; ++i) {
-        const int b = j * NG + (isv ? i / (D / 32) * 2 + (part >> 1) : i % NG);
-        const int dim = i % (D / 32) * 32 + r8;  // V
-        unsigned char* p = dst + i * 4096;
+        const int pi = i * (SR / 32) + rp;       // K: panel over (chunk of dims, block)
+        const int b = j * NG + (isv ? i / (D / SR) * 2 + (part >> 1) : pi % NG);
+        const int dim = i % (D / SR) * SR + r0s;  // V
+        unsigned char* p = dst + i * (SR * 128);
         if (b < nf) {
           put(p, *reinterpret_cast<const uint4*>(
                      isv ? vc + (long long)b * (D * kKV8Block) + dim * kKV8Block + (part & 1) * 16
-                         : kc + ((long long)b * NP + i / NG) * kKV8Panel + r8 * 64 + part * 16));
+                         : kc + ((long long)b * NP + pi / NG) * kKV8Panel + r8 * 64 + part * 16));
           continue;
         }
         const float up = s->tail[isv ? 2 : 0];
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(160 + 128 * NT, 1) attn_prefill_kv8_kernel(Att
           for (int q = 0; q < 2; ++q) {
             const int key = isv ? (part & 1) * 16 + e * 2 + q : r8;
             f[q] = b != nf || key >= tl ? 0.f
-                   : up * __bfloat162float(isv ? vt[dim * kKV8Block + key] : kt[(i / NG * kKV8Block + key) * 64 + part * 16 + e * 2 + q]);
+                   : up * __bfloat162float(isv ? vt[dim * kKV8Block + key] : kt[(pi / NG * kKV8Block + key) * 64 + part * 16 + e * 2 + q]);
           }
           *reinterpret_cast<uint32_t*>(p + (e < 4 ? w0 : w1) + (e & 3) * 4) = pack_f16x2(f[0], f[1]);
         }
@@ -271,7 +275,7 @@ __global__ void __launch_bounds__(160 + 128 * NT, 1) attn_prefill_kv8_kernel(Att
       unsigned char* dst = reinterpret_cast<unsigned char*>(tile);
       if (whole(j)) {
 #pragma unroll
-        for (int i = 0; i < PC; ++i) put(dst + i * 4096, x[i]);
+        for (int i = 0; i < PC; ++i) put(dst + i * (SR * 128), x[i]);
       } else {
         put_ragged(j, isv, dst);
       }
@@ -348,36 +352,49 @@ __global__ void __launch_bounds__(160 + 128 * NT, 1) attn_prefill_kv8_kernel(Att
   } else {
     // ------------------------------------ softmax ------------------------------------------------
     const int q = warp & 3;              // TMEM lane quarter of this warp
-    const int u = (warp - 4) >> 2;       // tile
+    const int u = (warp - CW) >> 2;      // tile
     const int row = q * 32 + lane, r = r0 + u * 128 + row;
     const bool live = r < R;
     const int t = live ? r / G : a.T - 1, hq = h * G + (live ? r % G : 0), pos = a.p0 + t;
     const uint32_t lane_at = (uint32_t)(q * 32) << 16;
-    float qs;  // score factor of the row
+    // The warp brings in its 32 rows, 8 dims to a lane and RI rows at a time; lane i keeps row i's
+    // score factor.
+    float qs = 0.f;
     {
-      const __nv_bfloat16* src = a.q + t * a.ldq + (long long)hq * D;
-      float mag = 0.f;
-      float f[16];
+      constexpr int LR = D / 8, RI = 32 / LR;
+      const int ld = lane % LR, lr = lane / LR;  // 8 dims from 8 ld of row lr of a step
+      const long long mine = live ? t * a.ldq + (long long)hq * D : -1;  // lane i: row i
+      unsigned char* base = reinterpret_cast<unsigned char*>(s->Q[u]) + (ld >> 3) * (128 * 128) + q * 32 * 128;
 #pragma unroll 1
-      for (int d = 0; d < D; d += 16) {
-        load16(src, d, a.vec_q, f);
+      for (int b = 0; b < LR; b += 8) {
+        uint4 x[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mag = fmaxf(mag, kv8_mag(f[e]));
-      }
-      float up, down;
-      pow2_scale(mag, &up, &down);
-      qs = a.sl2 * down;
-      unsigned char* base = reinterpret_cast<unsigned char*>(s->Q[u]) + row * 128;
-#pragma unroll 1
-      for (int d = 0; d < D; d += 16) {
-        load16(src, d, a.vec_q, f);
-        uint32_t y[8];
+        for (int k = 0; k < 8; ++k) {
+          const long long off = __shfl_sync(0xffffffffu, mine, (b + k) * RI + lr);
+          x[k] = off >= 0 ? load8_raw(a.q + off, ld * 8, a.vec_q) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        uint32_t mx[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = live ? pack_f16x2(f[2 * e] * up, f[2 * e + 1] * up) : 0u;
-        unsigned char* p = base + (d >> 6) * (128 * 128);
-        const int un = (d & 63) >> 3;
-        *reinterpret_cast<uint4*>(p + ((un ^ (row & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(p + (((un + 1) ^ (row & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+        for (int k = 0; k < 8; ++k) {
+          mx[k] = kv8_max2_finite(kv8_max2_finite(kv8_max2_finite(kv8_max2_finite(0u, x[k].x), x[k].y), x[k].z), x[k].w);
+          mx[k] = max(mx[k] & 0xffffu, mx[k] >> 16);
+        }
+#pragma unroll
+        for (int o = 1; o < LR; o <<= 1)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mx[k] = max(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], o));
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int rw = (b + k) * RI + lr;
+          float up, down, f[8];
+          pow2_scale(kv8_bits(mx[k]), &up, &down);
+          const float back = __shfl_sync(0xffffffffu, down, lane % RI * LR);  // row lane % RI of this step
+          if (lane / RI == b + k) qs = a.sl2 * back;
+          unpack8(*reinterpret_cast<const bf16x8*>(&x[k]), f);
+          *reinterpret_cast<uint4*>(base + rw * 128 + (((ld & 7) ^ (rw & 7)) << 4)) =
+              make_uint4(pack_f16x2(f[0] * up, f[1] * up), pack_f16x2(f[2] * up, f[3] * up),
+                         pack_f16x2(f[4] * up, f[5] * up), pack_f16x2(f[6] * up, f[7] * up));
+        }
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
@@ -553,7 +570,7 @@ static cudaError_t launch_prefill(const AttnPrefillKV8Args& a, cudaStream_t st) 
   if (e != cudaSuccess) return e;
   const int R = a.T * (a.Hq / a.c.Hkv);
   e = hx_launch_pdl(k, dim3((unsigned)a.c.Hkv, (unsigned)((R + 128 * NT - 1) / (128 * NT)), (unsigned)a.splits),
-                    dim3(160 + 128 * NT), smem, st, a);
+                    dim3(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 * NT), smem, st, a);
   if (e != cudaSuccess || a.splits == 1) return e;
   return hx_launch_pdl(attn_prefill_kv8_merge<D>, dim3((unsigned)(((long long)a.c.Hkv * R + 3) / 4)), dim3(128), 0, st, a);
 }
