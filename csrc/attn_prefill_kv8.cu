@@ -16,7 +16,8 @@
 //                    memory, in the 128-byte-swizzled layout the MMA reads (2-stage rings for K, V);
 //   next 4 NT warps  softmax, a thread a row: scores from TMEM, running max with a lazy rescale of O
 //                    (only when the max grows by more than 2^8), P as f16 back into the score
-//                    columns of TMEM, from where it is the A operand of P V;
+//                    columns of TMEM, from where it is the A operand of P V. q lies in TMEM too: with
+//                    both left operands there, a product reads half the shared memory;
 //   last warp        issues the MMAs from one thread. Score buffers alternate (the two tiles', or
 //                    two of one tile), so the tensor cores work on one while the other is in softmax.
 // With few rows the keys are split over CTAs and their (O, max, sum) merged by a second kernel.
@@ -65,20 +66,19 @@ HX_DEVICE void tmem_st32(uint32_t taddr, const uint32_t* v) {
 }
 HX_DEVICE void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D[tmem] (+)= A[smem] * B[smem]^T and D[tmem] (+)= A[tmem] * B[smem]^T, f16 inputs, f32 accumulate.
-HX_DEVICE void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
-}
+// D[tmem] (+)= A[tmem] * B[smem]^T, f16 inputs (two to a column of A), f32 accumulate.
 HX_DEVICE void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
+}
+// One lane of a converged warp.
+HX_DEVICE bool elect_one() {
+  uint32_t y;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(y));
+  return y != 0;
 }
 HX_DEVICE constexpr uint32_t idesc_f16_f32(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);  // f32 accumulator, f16 A and B
@@ -112,28 +112,31 @@ HX_DEVICE void finish16(const AttnPrefillKV8Args& a, int t, int hq, int d0, floa
 template <int D, int NT, int BN>
 struct PrefillKV8Smem {
   static constexpr int CW = NT == 1 ? 8 : 4;  // converter warps
-  alignas(1024) __half Q[NT][128 * D];  // per tile: D/64 chunks of [128 rows x 64], 128B-swizzled
-  alignas(1024) __half K[2][BN * D];    // per stage: D/64 chunks of [BN keys x 64 dims]
-  alignas(1024) __half V[2][BN * D];    // per stage: BN/64 chunks of [D dims x 64 keys]
-  float kmul[4][BN / 32];               // tile j at j % 4: score factor of each 32 keys,
-  float vadd[4][BN / 32];               // log2(vs / vref) and its inverse factor
-  float vinv[4][BN / 32];
+  static constexpr int ST = BN * D <= 128 * 64 ? 4 : 2;  // stages of the K and V rings
+  static constexpr int SC = 2 * ST;           // tiles whose scales are held
+  alignas(1024) __half Q[NT][128 * D];  // rows of q on their way to TMEM: D/64 chunks of [128 rows x 64], swizzled
+  alignas(1024) __half K[ST][BN * D];    // per stage: D/64 chunks of [BN keys x 64 dims]
+  alignas(1024) __half V[ST][BN * D];    // per stage: BN/64 chunks of [D dims x 64 keys]
+  float kmul[SC][BN / 32];              // tile j at j % SC: score factor of each 32 keys,
+  float vadd[SC][BN / 32];              // log2(vs / vref) and its inverse factor
+  float vinv[SC][BN / 32];
   float red[3][16];
   float tail[4];                        // K tail: up, down; V tail: up, down
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], sc_full[4], s_full[2], p_full[2], o_done[NT];
+  uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], sc_full[SC], s_full[2], p_full[2], o_done[NT];
   uint32_t tmem_base;
   int abort;
 };
 
 template <int D, int NT, int BN, bool FP8>
 __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 * NT, 1) attn_prefill_kv8_kernel(AttnPrefillKV8Args a) {
-  static_assert(NT * D + 2 * BN <= 512, "TMEM: the tiles' O and two score buffers");
+  static_assert(NT * D + 2 * BN + NT * D / 2 <= 512, "TMEM: the tiles' O, two score buffers, q");
   using SM = PrefillKV8Smem<D, NT, BN>;
   constexpr int CW = SM::CW, MMA_WARP = CW + 4 * NT, NTH = 32 * (MMA_WARP + 1), NG = BN / 32, NP = D / 64;
-  constexpr uint32_t S_COL = NT * D;
+  constexpr uint32_t S_COL = NT * D, Q_COL = S_COL + 2 * BN;
+  constexpr int ST = SM::ST, SC = SM::SC;
   extern __shared__ __align__(1024) unsigned char raw[];
   SM* s = reinterpret_cast<SM*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int h = blockIdx.x, G = a.Hq / a.c.Hkv, R = a.T * G, L = a.p0 + a.T, nf = L / kKV8Block;
   const int r0 = (gridDim.y - 1 - blockIdx.y) * 128 * NT;  // the longest rows first
   const int kend = a.p0 + (min(r0 + 128 * NT, R) - 1) / G + 1;  // keys that any of the CTA's rows sees
@@ -142,15 +145,17 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
 
   if (tid == 0) {
     tc::mbar_init(&s->q_full, 4 * NT);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < ST; ++i) {
       tc::mbar_init(&s->k_full[i], CW);
       tc::mbar_init(&s->k_empty[i], 1);
       tc::mbar_init(&s->v_full[i], CW);
       tc::mbar_init(&s->v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&s->s_full[i], 1);
       tc::mbar_init(&s->p_full[i], 4);
     }
-    for (int i = 0; i < 4; ++i) tc::mbar_init(&s->sc_full[i], 1);
+    for (int i = 0; i < SC; ++i) tc::mbar_init(&s->sc_full[i], 1);
     for (int i = 0; i < NT; ++i) tc::mbar_init(&s->o_done[i], 1);
     s->abort = 0;
     tc::fence_barrier_init();
@@ -280,27 +285,37 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
         put_ragged(j, isv, dst);
       }
     };
-    if (nb > 0) load_k(jb);
+    float k1 = 0.f, v1 = 0.f;  // threads 0 .. NG-1: the next tile's scales
+    auto load_scales = [&](int j) {
+      const int b = j * NG + tid;
+      if (tid >= NG) return;
+      k1 = b < nf ? ks[b] : b == nf && tl ? s->tail[1] : 0.f;
+      v1 = b < nf ? vs[b] : b == nf && tl ? s->tail[3] : 0.f;
+    };
+    if (nb > 0) {
+      load_k(jb);
+      load_scales(jb);
+    }
     for (int i = 0; i < nb; ++i) {
-      const int j = jb + i, st = i & 1;
+      const int j = jb + i, st = i % ST;
       load_v(j);
-      if (i >= 2) ok = tc::mbar_wait(&s->k_empty[st], ((i >> 1) - 1) & 1, a.err, 7001);
+      if (i >= ST) ok = tc::mbar_wait(&s->k_empty[st], (i / ST - 1) & 1, a.err, 7001);
       if (!__all_sync(0xffffffffu, ok) || *(volatile int*)&s->abort) break;
       store(j, false, xk, s->K[st]);
       if (tid < NG) {
-        const int b = j * NG + tid;
-        const float k1 = b < nf ? ks[b] : b == nf && tl ? s->tail[1] : 0.f;
-        const float v1 = b < nf ? vs[b] : b == nf && tl ? s->tail[3] : 0.f;
-        s->kmul[i & 3][tid] = k1 > 0.f ? k1 : 1.f;  // a block of zeros: any factor
-        s->vadd[i & 3][tid] = v1 > 0.f ? log2f(v1 / vref) : 0.f;
-        s->vinv[i & 3][tid] = v1 > 0.f ? vref / v1 : 1.f;
+        s->kmul[i % SC][tid] = k1 > 0.f ? k1 : 1.f;  // a block of zeros: any factor
+        s->vadd[i % SC][tid] = v1 > 0.f ? log2f(v1 / vref) : 0.f;
+        s->vinv[i % SC][tid] = v1 > 0.f ? vref / v1 : 1.f;
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&s->k_full[st]);
-      if (tid == 0) tc::mbar_arrive(&s->sc_full[i & 3]);
-      if (i + 1 < nb) load_k(j + 1);
-      if (i >= 2) ok = tc::mbar_wait(&s->v_empty[st], ((i >> 1) - 1) & 1, a.err, 7002);
+      if (tid == 0) tc::mbar_arrive(&s->sc_full[i % SC]);
+      if (i + 1 < nb) {
+        load_k(j + 1);
+        load_scales(j + 1);
+      }
+      if (i >= ST) ok = tc::mbar_wait(&s->v_empty[st], (i / ST - 1) & 1, a.err, 7002);
       if (!__all_sync(0xffffffffu, ok) || *(volatile int*)&s->abort) break;
       store(j, true, xv, s->V[st]);
       tc::fence_proxy_async_smem();
@@ -310,35 +325,50 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
     if (!ok) s->abort = 1;
   } else if (warp == MMA_WARP) {
     // ------------------------------------ MMA issuer ---------------------------------------------
-    if (lane == 0 && nb > 0) {
+    // The whole warp runs the loop and one elected lane issues: addresses stay warp-uniform, which
+    // the MMA's operands have to be (issued from a divergent branch each cost about 90 cycles).
+    if (nb > 0) {
       constexpr uint32_t id_s = idesc_f16_f32(128, BN), id_o = idesc_f16_f32(128, D);
       const int items = nb * NT;  // item i: tile i % NT, key tile i / NT, score buffer i % 2
-      bool ok = tc::mbar_wait(&s->q_full, 0, a.err, 7003);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t kd = tc::sdesc_k128(__shfl_sync(0xffffffffu, tc::smem_u32(s->K[0]), 0));
+      const uint64_t vd = tc::sdesc_k128(__shfl_sync(0xffffffffu, tc::smem_u32(s->V[0]), 0));
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+        return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, a.err, code));
+      };
+      bool ok = wait(&s->q_full, 0, 7003);
       auto qk = [&](int i) {
-        const int j = i / NT, u = i % NT, st = j & 1;
-        if (u == 0 && !tc::mbar_wait(&s->k_full[st], (j >> 1) & 1, a.err, 7004)) return false;
+        const int j = i / NT, u = i % NT, st = j % ST;
+        if (u == 0 && !wait(&s->k_full[st], (j / ST) & 1, 7004)) return false;
         tc::tc_fence_after();
-        const uint32_t q0 = tc::smem_u32(s->Q[u]), k0 = tc::smem_u32(s->K[st]);
+        const uint64_t k0 = kd + st * (BN * D * 2 / 16);
+        const uint32_t d = tm + S_COL + (i & 1) * BN, q = tm + Q_COL + u * (D / 2);
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          umma_f16_ss(tmem + S_COL + (i & 1) * BN, tc::sdesc_k128(q0 + (k >> 2) * 128 * 128 + (k & 3) * 32),
-                      tc::sdesc_k128(k0 + (k >> 2) * BN * 128 + (k & 3) * 32), id_s, k > 0);
-        tc::umma_commit(&s->s_full[i & 1]);
-        if (u == NT - 1) tc::umma_commit(&s->k_empty[st]);
+          for (int k = 0; k < D / 16; ++k)
+            umma_f16_ts(d, q + k * 8, k0 + (k >> 2) * (BN * 128 / 16) + (k & 3) * 2, id_s, k > 0);
+          tc::umma_commit(&s->s_full[i & 1]);
+          if (u == NT - 1) tc::umma_commit(&s->k_empty[st]);
+        }
+        __syncwarp();
         return true;
       };
       auto pv = [&](int i) {
-        const int j = i / NT, u = i % NT, st = j & 1;
-        if (u == 0 && !tc::mbar_wait(&s->v_full[st], (j >> 1) & 1, a.err, 7005)) return false;
-        if (!tc::mbar_wait(&s->p_full[i & 1], (i >> 1) & 1, a.err, 7006)) return false;
+        const int j = i / NT, u = i % NT, st = j % ST;
+        if (u == 0 && !wait(&s->v_full[st], (j / ST) & 1, 7005)) return false;
+        if (!wait(&s->p_full[i & 1], (i >> 1) & 1, 7006)) return false;
         tc::tc_fence_after();
-        const uint32_t v0 = tc::smem_u32(s->V[st]);
+        const uint64_t v0 = vd + st * (BN * D * 2 / 16);
+        const uint32_t d = tm + u * D, p = tm + S_COL + (i & 1) * BN;
+        const uint32_t more = j > 0 ? 1u : 0u;
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < BN / 16; ++k)
-          umma_f16_ts(tmem + u * D, tmem + S_COL + (i & 1) * BN + k * 8,
-                      tc::sdesc_k128(v0 + (k >> 2) * D * 128 + (k & 3) * 32), id_o, (j > 0 || k > 0) ? 1u : 0u);
-        tc::umma_commit(&s->o_done[u]);
-        if (u == NT - 1) tc::umma_commit(&s->v_empty[st]);
+          for (int k = 0; k < BN / 16; ++k)
+            umma_f16_ts(d, p + k * 8, v0 + (k >> 2) * (D * 128 / 16) + (k & 3) * 2, id_o, k > 0 ? 1u : more);
+          tc::umma_commit(&s->o_done[u]);
+          if (u == NT - 1) tc::umma_commit(&s->v_empty[st]);
+        }
+        __syncwarp();
         return true;
       };
       ok = ok && qk(0);
@@ -347,7 +377,7 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
         if (i + 1 < items) ok = qk(i + 1);
         ok = ok && pv(i);
       }
-      if (!ok) s->abort = 1;
+      if (!ok && lane == 0) s->abort = 1;
     }
   } else {
     // ------------------------------------ softmax ------------------------------------------------
@@ -396,7 +426,20 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
                          pack_f16x2(f[4] * up, f[5] * up), pack_f16x2(f[6] * up, f[7] * up));
         }
       }
-      tc::fence_proxy_async_smem();
+      __syncwarp();
+#pragma unroll 1
+      for (int c = 0; c < D / 64; ++c) {  // each thread its own row, 64 dims to 32 columns
+        const unsigned char* p = reinterpret_cast<const unsigned char*>(s->Q[u]) + c * (128 * 128) + row * 128;
+        uint32_t y[32];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint4 x = *reinterpret_cast<const uint4*>(p + ((e ^ (row & 7)) << 4));
+          y[4 * e] = x.x; y[4 * e + 1] = x.y; y[4 * e + 2] = x.z; y[4 * e + 3] = x.w;
+        }
+        tmem_st32(tmem + lane_at + Q_COL + u * (D / 2) + c * 32, y);
+      }
+      tmem_wait_st();
+      tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&s->q_full);
     }
@@ -406,9 +449,9 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
     for (int j = 0; j < nb; ++j) {
       const int i = j * NT + u, sl = i & 1;
       if (!__all_sync(0xffffffffu, tc::mbar_wait(&s->s_full[sl], (i >> 1) & 1, a.err, 7007))) { ok = false; break; }
-      // The tile's scale factors. Tile j + 4 overwrites them after P_j was consumed, so this wait
+      // The tile's scale factors. Tile j + SC overwrites them after P_j was consumed, so this wait
       // is never more than one phase behind (k_full, refilled after Q K_j, could be two).
-      if (!__all_sync(0xffffffffu, tc::mbar_wait(&s->sc_full[j & 3], (j >> 2) & 1, a.err, 7008))) { ok = false; break; }
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(&s->sc_full[j % SC], (j / SC) & 1, a.err, 7008))) { ok = false; break; }
       tc::tc_fence_after();
       const uint32_t sa = tmem + lane_at + S_COL + sl * BN;
       const int k0 = (jb + j) * BN;
@@ -417,7 +460,7 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
       float km[NG];
       float mx = -INFINITY;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) km[g] = s->kmul[j & 3][g] * qs;
+      for (int g = 0; g < NG; ++g) km[g] = s->kmul[j % SC][g] * qs;
 #pragma unroll
       for (int c = 0; c < BN / 64; ++c) {
         float x[64];
@@ -467,7 +510,7 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
         uint32_t y[32];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const float b = s->vadd[j & 3][c * 2 + g] - base;
+          const float b = s->vadd[j % SC][c * 2 + g] - base;
           float sum = 0.f;
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
@@ -476,7 +519,7 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
             sum += p0 + p1;
             y[g * 16 + e / 2] = pack_f16x2(p0, p1);
           }
-          l = fmaf(sum, s->vinv[j & 3][c * 2 + g], l);
+          l = fmaf(sum, s->vinv[j % SC][c * 2 + g], l);
         }
         tmem_st32(sa + c * 32, y);  // over scores that this thread has read twice
       }
@@ -582,7 +625,7 @@ cudaError_t attn_prefill_kv8_launch(const AttnPrefillKV8Args& a, cudaStream_t st
     constexpr bool F = decltype(fp8)::value;
     if constexpr (D == 256) e = launch_prefill<256, 1, 64, F>(a, st);
     else if (a.NT == 1) e = launch_prefill<D, 1, 128, F>(a, st);
-    else e = launch_prefill<D, 2, 128, F>(a, st);
+    else e = launch_prefill<D, 2, D == 128 ? 64 : 128, F>(a, st);
   });
   return e;
 }
