@@ -66,7 +66,15 @@ HX_DEVICE void tmem_st32(uint32_t taddr, const uint32_t* v) {
 }
 HX_DEVICE void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D[tmem] (+)= A[tmem] * B[smem]^T, f16 inputs (two to a column of A), f32 accumulate.
+// D[tmem] (+)= A * B[smem]^T with A in shared memory or in TMEM (two f16 to a column), f16 inputs,
+// f32 accumulate.
+HX_DEVICE void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
 HX_DEVICE void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -112,9 +120,10 @@ HX_DEVICE void finish16(const AttnPrefillKV8Args& a, int t, int hq, int d0, floa
 template <int D, int NT, int BN>
 struct PrefillKV8Smem {
   static constexpr int CW = NT == 1 ? 8 : 4;  // converter warps
+  static constexpr bool QT = NT * D + 2 * BN + NT * D / 2 <= 512;  // q fits TMEM beside O and the scores
   static constexpr int ST = BN * D <= 128 * 64 ? 4 : 2;  // stages of the K and V rings
   static constexpr int SC = 2 * ST;           // tiles whose scales are held
-  alignas(1024) __half Q[NT][128 * D];  // rows of q on their way to TMEM: D/64 chunks of [128 rows x 64], swizzled
+  alignas(1024) __half Q[NT][128 * D];  // rows of q (on their way to TMEM if QT): D/64 chunks of [128 rows x 64], swizzled
   alignas(1024) __half K[ST][BN * D];    // per stage: D/64 chunks of [BN keys x 64 dims]
   alignas(1024) __half V[ST][BN * D];    // per stage: BN/64 chunks of [D dims x 64 keys]
   float kmul[SC][BN / 32];              // tile j at j % SC: score factor of each 32 keys,
@@ -129,11 +138,12 @@ struct PrefillKV8Smem {
 
 template <int D, int NT, int BN, bool FP8>
 __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 * NT, 1) attn_prefill_kv8_kernel(AttnPrefillKV8Args a) {
-  static_assert(NT * D + 2 * BN + NT * D / 2 <= 512, "TMEM: the tiles' O, two score buffers, q");
+  static_assert(NT * D + 2 * BN <= 512, "TMEM: the tiles' O and two score buffers");
   using SM = PrefillKV8Smem<D, NT, BN>;
   constexpr int CW = SM::CW, MMA_WARP = CW + 4 * NT, NTH = 32 * (MMA_WARP + 1), NG = BN / 32, NP = D / 64;
   constexpr uint32_t S_COL = NT * D, Q_COL = S_COL + 2 * BN;
   constexpr int ST = SM::ST, SC = SM::SC;
+  constexpr bool QT = SM::QT;
   extern __shared__ __align__(1024) unsigned char raw[];
   SM* s = reinterpret_cast<SM*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -285,6 +295,8 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
         put_ragged(j, isv, dst);
       }
     };
+    // (approximate log2 and quotient: 2^vadd * vinv stays 1 to 2^-20, a probability has 11 bits)
+    const float vdown = 1.f / vref;
     float k1 = 0.f, v1 = 0.f;  // threads 0 .. NG-1: the next tile's scales
     auto load_scales = [&](int j) {
       const int b = j * NG + tid;
@@ -304,8 +316,8 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
       store(j, false, xk, s->K[st]);
       if (tid < NG) {
         s->kmul[i % SC][tid] = k1 > 0.f ? k1 : 1.f;  // a block of zeros: any factor
-        s->vadd[i % SC][tid] = v1 > 0.f ? log2f(v1 / vref) : 0.f;
-        s->vinv[i % SC][tid] = v1 > 0.f ? vref / v1 : 1.f;
+        s->vadd[i % SC][tid] = v1 > 0.f ? __log2f(v1 * vdown) : 0.f;
+        s->vinv[i % SC][tid] = v1 > 0.f ? __fdividef(vref, v1) : 1.f;
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
@@ -332,6 +344,7 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
       const int items = nb * NT;  // item i: tile i % NT, key tile i / NT, score buffer i % 2
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint64_t kd = tc::sdesc_k128(__shfl_sync(0xffffffffu, tc::smem_u32(s->K[0]), 0));
+      const uint64_t qd = tc::sdesc_k128(__shfl_sync(0xffffffffu, tc::smem_u32(s->Q[0]), 0));
       const uint64_t vd = tc::sdesc_k128(__shfl_sync(0xffffffffu, tc::smem_u32(s->V[0]), 0));
       auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
         return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, a.err, code));
@@ -341,12 +354,13 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
         const int j = i / NT, u = i % NT, st = j % ST;
         if (u == 0 && !wait(&s->k_full[st], (j / ST) & 1, 7004)) return false;
         tc::tc_fence_after();
-        const uint64_t k0 = kd + st * (BN * D * 2 / 16);
+        const uint64_t k0 = kd + st * (BN * D * 2 / 16), q0 = qd + u * (128 * D * 2 / 16);
         const uint32_t d = tm + S_COL + (i & 1) * BN, q = tm + Q_COL + u * (D / 2);
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            umma_f16_ts(d, q + k * 8, k0 + (k >> 2) * (BN * 128 / 16) + (k & 3) * 2, id_s, k > 0);
+            if constexpr (QT) umma_f16_ts(d, q + k * 8, k0 + (k >> 2) * (BN * 128 / 16) + (k & 3) * 2, id_s, k > 0);
+            else umma_f16_ss(d, q0 + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2, k0 + (k >> 2) * (BN * 128 / 16) + (k & 3) * 2, id_s, k > 0);
           tc::umma_commit(&s->s_full[i & 1]);
           if (u == NT - 1) tc::umma_commit(&s->k_empty[st]);
         }
@@ -426,20 +440,24 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
                          pack_f16x2(f[4] * up, f[5] * up), pack_f16x2(f[6] * up, f[7] * up));
         }
       }
-      __syncwarp();
+      if constexpr (QT) {
+        __syncwarp();
 #pragma unroll 1
-      for (int c = 0; c < D / 64; ++c) {  // each thread its own row, 64 dims to 32 columns
-        const unsigned char* p = reinterpret_cast<const unsigned char*>(s->Q[u]) + c * (128 * 128) + row * 128;
-        uint32_t y[32];
+        for (int c = 0; c < D / 64; ++c) {  // each thread its own row, 64 dims to 32 columns
+          const unsigned char* p = reinterpret_cast<const unsigned char*>(s->Q[u]) + c * (128 * 128) + row * 128;
+          uint32_t y[32];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint4 x = *reinterpret_cast<const uint4*>(p + ((e ^ (row & 7)) << 4));
-          y[4 * e] = x.x; y[4 * e + 1] = x.y; y[4 * e + 2] = x.z; y[4 * e + 3] = x.w;
+          for (int e = 0; e < 8; ++e) {
+            const uint4 x = *reinterpret_cast<const uint4*>(p + ((e ^ (row & 7)) << 4));
+            y[4 * e] = x.x; y[4 * e + 1] = x.y; y[4 * e + 2] = x.z; y[4 * e + 3] = x.w;
+          }
+          tmem_st32(tmem + lane_at + Q_COL + u * (D / 2) + c * 32, y);
         }
-        tmem_st32(tmem + lane_at + Q_COL + u * (D / 2) + c * 32, y);
+        tmem_wait_st();
+        tc::tc_fence_before();
+      } else {
+        tc::fence_proxy_async_smem();
       }
-      tmem_wait_st();
-      tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&s->q_full);
     }
@@ -604,6 +622,7 @@ __global__ void __launch_bounds__(128) attn_prefill_kv8_merge(AttnPrefillKV8Args
   }
 }
 
+constexpr int kBN128 = 128;
 template <int D, int NT, int BN, bool FP8>
 static cudaError_t launch_prefill(const AttnPrefillKV8Args& a, cudaStream_t st) {
   auto k = attn_prefill_kv8_kernel<D, NT, BN, FP8>;
@@ -625,7 +644,7 @@ cudaError_t attn_prefill_kv8_launch(const AttnPrefillKV8Args& a, cudaStream_t st
     constexpr bool F = decltype(fp8)::value;
     if constexpr (D == 256) e = launch_prefill<256, 1, 64, F>(a, st);
     else if (a.NT == 1) e = launch_prefill<D, 1, 128, F>(a, st);
-    else e = launch_prefill<D, 2, D == 128 ? 64 : 128, F>(a, st);
+    else e = launch_prefill<D, 2, kBN128, F>(a, st);
   });
   return e;
 }
