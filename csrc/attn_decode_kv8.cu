@@ -8,7 +8,7 @@
 // tensor cores over codes, and the scales are f32 factors outside them.
 //
 // Work is laid out as one list of blocks (32 keys of one sequence and kv head) over the whole
-// ragged batch. Clusters of kCL CTAs take equal runs of it, so sequences of any mix of lengths
+// ragged batch. CTAs, or clusters of four, take equal runs of it, so sequences of any mix of lengths
 // load every SM alike; a run may end inside a pair (sequence, kv head) and go on into the next.
 // Inside a run's part of one pair (a segment) every warp of the cluster takes whole blocks, a
 // warp with its own ring of bulk copies: K and V blocks are contiguous panels, so a copy is one
@@ -44,16 +44,18 @@ struct KV8Ring {
   static constexpr int kSlots = D >= 128 ? 5 : 8;                 // slots of a warp's ring
 };
 
-template <int D, int NT>
+template <int D, int NT, int CL>
 struct DecodeKV8Smem {
+  static constexpr int kMaxPart = CL == 1 ? kKV8MaxCtas : kKV8MaxCtas / CL;  // most partials of a pair
   static constexpr int GP = NT * 8;      // heads of a pass, padded
   static constexpr int LD = D + 4;       // row stride of wo: lanes of one store hit distinct banks
   union {
     alignas(128) uint8_t ring[kKV8Warps][KV8Ring<D>::kSlots][KV8Ring<D>::kUnit];
     alignas(16) float wo[kKV8Warps][GP][LD];  // the warps' O, then (in [0]) the CTA's
-    float fw[GP][kKV8MaxPart];           // the partials' weights in the last merge
+    float fw[GP][kMaxPart];              // the partials' weights in the last merge
   };
   alignas(16) float q[GP][D];            // normed, rotated, times a power of two
+  alignas(16) float kn[D];               // the new key
   alignas(16) uint2 qf[NT][D / 16][32];  // the same as f16 operands, a lane's four values together
   alignas(16) __nv_bfloat16 knew[D], vnew[D];  // the new token as the cache holds it
   float ps[kKV8Warps][2 * NT][32][4];    // the warps' parts of the last block's scores
@@ -67,7 +69,8 @@ struct DecodeKV8Smem {
   int off[kKV8MaxBatch + 1];             // blocks before sequence b
   int slot[kKV8MaxBatch], pos[kKV8MaxBatch];
   int nbmax;
-  float red[2][kKV8Warps], inv[2], scale[2];
+  uint32_t red[2][kKV8Warps];
+  float inv[2], scale[2];
   int last;
 };
 
@@ -246,18 +249,24 @@ HX_DEVICE void add4(float4& o, const float4& v, float f) {
   o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
 }
 
-template <int D, int NT, bool FP8>
+template <int D, int NT, int CL, bool FP8>
 __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(AttnDecodeKV8Args a) {
   using R = KV8Ring<D>;
-  using SM = DecodeKV8Smem<D, NT>;
+  using SM = DecodeKV8Smem<D, NT, CL>;
   constexpr int GP = SM::GP, NP = D / 64, NW = kKV8Warps, NTH = NW * 32;
   extern __shared__ __align__(128) unsigned char raw[];
   SM* s = reinterpret_cast<SM*>(raw);
-  cg::cluster_group cluster = cg::this_cluster();
-  constexpr int CL = kKV8CL;
-  const int crank = (int)cluster.block_rank(), cid = blockIdx.x / CL, NC = gridDim.x / CL;
+  const int crank = CL == 1 ? 0 : (int)cg::this_cluster().block_rank(), cid = blockIdx.x / CL, NC = gridDim.x / CL;
+  auto all_sync = [] {  // the cluster's threads
+    if constexpr (CL == 1) __syncthreads();
+    else cg::this_cluster().sync();
+  };
+  auto peer = [](auto* p, int x) {  // p in CTA x of the cluster
+    if constexpr (CL == 1) return p;
+    else return cg::this_cluster().map_shared_rank(p, x);
+  };
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int Hkv = a.c.Hkv, G = a.Hq / Hkv, HG = a.HG, per = (G + HG - 1) / HG, PB = Hkv * HG;
+  const int Hkv = a.c.Hkv, G = a.G, HG = a.HG, per = a.per, PB = Hkv * HG;
   const int qw = a.gated ? 2 * D : D;
   if (tid == 0) {
     for (int w = 0; w < NW; ++w)
@@ -338,7 +347,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
     const int pl = (w - s->off[b] * PB) / nb;  // kv head and head group
     const int p0 = s->off[b] * PB + pl * nb;   // the pair's first block in the list
     const int blk0 = w - p0, blk1 = min(nb, wend - p0);
-    const int pair = b * PB + pl, h = pl / HG, hg = pl % HG, g0 = hg * per, n = min(per, G - g0);
+    const int pair = b * PB + pl, h = HG == 1 ? pl : pl / HG, hg = pl - h * HG, g0 = hg * per, n = min(per, G - g0);
     const int slot = s->slot[b], p = s->pos[b], row = p % kKV8Block;
     const __nv_bfloat16* pr = a.proj + b * a.ldp;
     // ---- this warp's blocks: blk0 + gw, + CL * NW, ...; the sequence's last block is not copied --
@@ -370,22 +379,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       for (int i = 0; i < R::kSlots && todo > 0 && ok && lane == 0; ++i) issue();
     };
     if (!(completes && warp == host)) fill();
-    // ---- loads of all that the segment's start needs, in flight together -------------------------
-    const int nrow = n + (cta_last ? 1 : 0);  // the group's queries, then the new key
-    constexpr int NR = (GP + NW) / NW;
-    __nv_bfloat16 xr[NR][D / 32], xv[D / 32];
-#pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      const int r = warp + i * NW;
-      const __nv_bfloat16* src = r == n ? pr + a.Hq * qw + h * D : pr + (long long)(h * G + g0 + r) * qw;
-      if (r < nrow)
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) xr[i][e] = src[e * 32 + lane];
-    }
-    const bool kwarp = cta_last && warp == n % NW;
-    if (kwarp)
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) xv[e] = pr[a.Hq * qw + (Hkv + h) * D + e * 32 + lane];
+    // ---- loads that the segment's start needs, in flight together --------------------------------
     // The last block's bf16 rows, for the whole CTA: for a completed block 16-value pieces of the
     // block's layout (X[i][0..1] of K, [2..3] of V); else operands: warp w takes dims groups
     // (of 16) w * NP + i of the sums and of the output.
@@ -414,65 +408,85 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         }
       }
     }
-    const int prot = p + (a.rope_delta ? a.rope_delta[slot] : 0);
-    if (const int i = tid; i < a.rot / 2) rotation((float)prot * freq, &s->sn[i], &s->cs[i]);
-    __syncthreads();
     // ---- q of the group's heads (and the new key): norm, rotation ------------------------------
+    // Rows go over D / 8 lanes each, 8 dims to a lane, in small loops: code that runs once a launch
+    // costs its fetch.
+    constexpr int LR = D / 8, RP = NTH / LR;  // lanes of a row, rows of a pass
+    const int nrow = n + (cta_last ? 1 : 0);  // the group's queries, then the new key
+    const int rr = tid / LR, d0 = tid % LR * 8;
+    auto row_max = [](auto x) {
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      const int r = warp + i * NW;
-      if (r >= nrow) break;
+      for (int o = 1; o < LR; o <<= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
+      return x;
+    };
+#pragma unroll 1
+    for (int r = rr; r - rr < nrow; r += RP) {
       const bool isk = r == n;
-      float v[D / 32];
-      float ss = 0.f;
+      const __nv_bfloat16* src = isk ? pr + a.Hq * qw + h * D : pr + (long long)(h * G + g0 + r) * qw;
+      const uint4 x = r < nrow ? load8_raw(src, d0, a.vec) : make_uint4(0u, 0u, 0u, 0u);
+      float f[8];
+      unpack8(*reinterpret_cast<const bf16x8*>(&x), f);
+      if (a.q_norm_w || a.k_norm_w) {  // (weights of an absent norm are 1, its factor too)
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) {
-        v[e] = __bfloat162float(xr[i][e]);
-        ss += v[e] * v[e];
+        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+#pragma unroll
+        for (int o = 1; o < LR; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = (isk ? a.k_norm_w : a.q_norm_w) ? rsqrtf(ss * (1.f / D) + a.eps) : 1.f;
+        const float* w = (isk ? s->wk : s->wq) + d0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= inv * w[e];
       }
-      if (isk ? a.k_norm_w : a.q_norm_w) {
-        const float inv = rsqrtf(warp_sum(ss) / D + a.eps);
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) v[e] *= inv * (isk ? s->wk : s->wq)[e * 32 + lane];
+      if (r < nrow) {
+        float4* dst = reinterpret_cast<float4*>((isk ? s->kn : s->q[r]) + d0);
+        dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+        dst[1] = make_float4(f[4], f[5], f[6], f[7]);
       }
-      const int half = a.rot / 2;
-      if (half) {
-        float* x = isk ? s->ps[warp][0][0] : s->q[r];  // D floats that only this warp uses
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) x[e * 32 + lane] = v[e];
-        __syncwarp();
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) {
-          const int d = e * 32 + lane;
-          if (d < a.rot) v[e] = d < half ? v[e] * s->cs[d] - x[d + half] * s->sn[d]
-                                         : v[e] * s->cs[d - half] + x[d - half] * s->sn[d - half];
+    }
+    if (cta_last && rr == 0)
+      *reinterpret_cast<uint4*>(s->vnew + d0) = load8_raw(pr + a.Hq * qw + (Hkv + h) * D, d0, a.vec);
+    const int half = a.rot / 2;
+    if (half) {
+      const int prot = p + (a.rope_delta ? a.rope_delta[slot] : 0);
+      if (tid < half) rotation((float)prot * freq, &s->sn[tid], &s->cs[tid]);
+      __syncthreads();
+#pragma unroll 1
+      for (int r = warp; r < nrow; r += NW) {
+        float* x = r == n ? s->kn : s->q[r];
+#pragma unroll 1
+        for (int i = lane; i < half; i += 32) {
+          const float lo = x[i], hi = x[i + half], cs = s->cs[i], sn = s->sn[i];
+          x[i] = lo * cs - hi * sn;
+          x[i + half] = hi * cs + lo * sn;
         }
-        __syncwarp();
       }
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int r = rr; r - rr < nrow; r += RP) {
+      const bool isk = r == n;
+      float4* x = reinterpret_cast<float4*>((isk ? s->kn : s->q[min(r, GP - 1)]) + d0);
+      const float4 y = x[0], z = x[1];
+      const float f[8] = {y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+      float mag = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mag = fmaxf(mag, kv8_mag(f[e]));
+      // power of two that brings the row's largest entry to 128..256
+      const int ex = min(134 - (int)(row_max(__float_as_uint(mag)) >> 23), 120);
+      const float up = __uint_as_float((uint32_t)(ex + 127) << 23);
       if (isk) {
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) {
-          s->knew[e * 32 + lane] = __float2bfloat16(v[e]);
-          s->vnew[e * 32 + lane] = xv[e];
+        *reinterpret_cast<bf16x8*>(s->knew + d0) = pack8(f);
+      } else if (r < n) {
+        const float u[8] = {f[0] * up, f[1] * up, f[2] * up, f[3] * up, f[4] * up, f[5] * up, f[6] * up, f[7] * up};
+        if (cta_last) {
+          x[0] = make_float4(u[0], u[1], u[2], u[3]);
+          x[1] = make_float4(u[4], u[5], u[6], u[7]);
         }
-      } else {
-        float mag = 0.f;
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) mag = fmaxf(mag, kv8_mag(v[e]));
-        mag = warp_max(mag);
-        // power of two that brings the largest entry to 128..256
-        const int ex = min(134 - (int)(__float_as_uint(mag) >> 23), 120);
-        const float up = __uint_as_float((uint32_t)(ex + 127) << 23);
-        __half* qf = reinterpret_cast<__half*>(s->qf[r >> 3]);
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) {
-          const int d = e * 32 + lane;
-          if (cta_last) s->q[r][d] = v[e] * up;
-          // lane 4 (r % 8) + (d / 16) % 4 of dims group 4 (d / 64) + (d / 4) % 4 holds d % 4
-          const int k = (d >> 6) * 4 + ((d >> 2) & 3), l = (r & 7) * 4 + ((d >> 4) & 3);
-          qf[(k * 32 + l) * 4 + (d & 3)] = __float2half_rn(v[e] * up);
-        }
-        if (lane == 0) s->qmul[r] = a.sl2 * __uint_as_float((uint32_t)(127 - ex) << 23);
+        // dims 4 (k % 4) + 16 t of panel k / 4 are lane 4 (r % 8) + t's in operand k
+        const int k = (d0 >> 6) * 4 + ((d0 >> 2) & 3), l = (r & 7) * 4 + ((d0 >> 4) & 3);
+        s->qf[r >> 3][k][l] = make_uint2(pack_f16x2(u[0], u[1]), pack_f16x2(u[2], u[3]));
+        s->qf[r >> 3][k + 1][l] = make_uint2(pack_f16x2(u[4], u[5]), pack_f16x2(u[6], u[7]));
+        if (d0 == 0) s->qmul[r] = a.sl2 * __uint_as_float((uint32_t)(127 - ex) << 23);
       }
     }
     __syncthreads();
@@ -502,7 +516,6 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       if (completes) {
         // Its codes, into the ring (that warp has no copies under way) and into the cache. Every
         // head group derives them; the first one stores them.
-        float mag[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
           const int c = i * NTH + tid;
@@ -513,24 +526,31 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
           }
           if (c & 1)  // key 31 of V's dim c / 2
             X[i][3].w = (X[i][3].w & 0xffffu) | (uint32_t)__bfloat16_as_ushort(s->vnew[c >> 1]) << 16;
+        }
+        uint32_t mag[2];
+        auto block_max = [&](auto max2) {  // of K and V over the CTA
+          mag[0] = mag[1] = 0u;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float f[8];
-            unpack8(*reinterpret_cast<const bf16x8*>(&X[i][q]), f);
+          for (int i = 0; i < NP; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mag[q >> 1] = fmaxf(mag[q >> 1], kv8_mag(f[e]));
+            for (int q = 0; q < 4; ++q)
+              mag[q >> 1] = max2(max2(max2(max2(mag[q >> 1], X[i][q].x), X[i][q].y), X[i][q].z), X[i][q].w);
+          __syncthreads();
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            mag[z] = kv8_max1(mag[z]);
+            if (lane == 0) s->red[z][warp] = mag[z];
           }
-        }
+          __syncthreads();
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          mag[z] = warp_max(mag[z]);
-          if (lane == 0) s->red[z][warp] = mag[z];
-        }
-        __syncthreads();
+          for (int z = 0; z < 2; ++z) mag[z] = max(max(s->red[z][0], s->red[z][1]), max(s->red[z][2], s->red[z][3]));
+        };
+        block_max([](uint32_t m, uint32_t x) { return kv8_max2(m, x); });
+        const bool special = max(mag[0], mag[1]) >= kKV8Inf;
+        if (special) block_max([](uint32_t m, uint32_t x) { return kv8_max2_finite(m, x); });
         const long long at = a.c.block(slot, h, nb - 1);
         if (tid < 2) {
-          const float m = fmaxf(fmaxf(s->red[tid][0], s->red[tid][1]), fmaxf(s->red[tid][2], s->red[tid][3]));
-          const float scale = kv8_scale<FP8>(m);
+          const float m = kv8_bits(tid ? mag[1] : mag[0]), scale = kv8_scale<FP8>(m);
           s->inv[tid] = kv8_inv<FP8>(m);
           s->scale[tid] = scale;
           if (hg == 0) (tid ? a.c.vs : a.c.ks)[at] = scale;
@@ -544,11 +564,8 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
           uint8_t* dst = (z ? a.c.vc : a.c.kc) + at * (D * kKV8Block);
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
-            float f[16];
-            unpack8(*reinterpret_cast<const bf16x8*>(&X[i][2 * z]), f);
-            unpack8(*reinterpret_cast<const bf16x8*>(&X[i][2 * z + 1]), f + 8);
-            const uint4 v = make_uint4(kv8_code4<FP8>(f, inv), kv8_code4<FP8>(f + 4, inv),
-                                       kv8_code4<FP8>(f + 8, inv), kv8_code4<FP8>(f + 12, inv));
+            const uint2 u = kv8_code8<FP8>(X[i][2 * z], inv, special), w = kv8_code8<FP8>(X[i][2 * z + 1], inv, special);
+            const uint4 v = make_uint4(u.x, u.y, w.x, w.y);
             reinterpret_cast<uint4*>(fresh + z * D * kKV8Block)[i * NTH + tid] = v;
             if (hg == 0) reinterpret_cast<uint4*>(dst)[i * NTH + tid] = v;
           }
@@ -770,7 +787,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       if (d == 0) { s->cm[r] = M; s->cl[r] = L; }
     }
     // ---- merge the cluster's CTAs: each finishes 1 / CL of the columns -------------------
-    cluster.sync();
+    all_sync();
     auto finish = [&](int r, int d, float4 o, float l) {  // four dims of the output
       const int hq = h * G + g0 + r;
       const float il = __fdividef(1.f, l);
@@ -794,9 +811,9 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       float4 v[CL], O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int x = 0; x < CL; ++x) {
-        m[x] = *cluster.map_shared_rank(&s->cm[r], x);
-        l[x] = *cluster.map_shared_rank(&s->cl[r], x);
-        v[x] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&s->wo[0][r][d], x));
+        m[x] = *peer(&s->cm[r], x);
+        l[x] = *peer(&s->cl[r], x);
+        v[x] = *reinterpret_cast<const float4*>(peer(&s->wo[0][r][d], x));
       }
 #pragma unroll
       for (int x = 0; x < CL; ++x) M = fmaxf(M, m[x]);
@@ -815,7 +832,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
     }
     if (!alone) __threadfence();
     tc::fence_proxy_async_smem();  // O's stores before the next segment's copies into the same memory
-    cluster.sync();
+    all_sync();
     if (!alone) {
       // the cluster that completes the pair's block count merges its partials
       if (crank == 0 && tid == 0) {
@@ -823,9 +840,9 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         const int last = atomicAdd(counter, blk1 - blk0) + (blk1 - blk0) == nb;
         if (last) *counter = 0;
         __threadfence();
-        for (int x = 0; x < CL; ++x) *cluster.map_shared_rank(&s->last, x) = last;
+        for (int x = 0; x < CL; ++x) *peer(&s->last, x) = last;
       }
-      cluster.sync();
+      all_sync();
       if (s->last) {
         __threadfence();
         const int f0 = p0 / chunk, np = (p0 + nb - 1) / chunk - f0 + 1;  // its clusters
@@ -833,7 +850,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         const int r0 = c0 / (D / 4), r1 = (c0 + cols - 1) / (D / 4);       // heads of this CTA's columns
 #pragma unroll 1
         for (int r = r0 + warp; r <= r1; r += NW) {
-          constexpr int NX = (kKV8MaxPart + 31) / 32;
+          constexpr int NX = (SM::kMaxPart + 31) / 32;
           float2 ml[NX];
           float M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -876,11 +893,11 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
   }
 }
 
-template <int D, int NT, bool FP8>
+template <int D, int NT, int CL, bool FP8>
 static cudaError_t launch_decode(AttnDecodeKV8Args a, cudaStream_t st) {
-  auto k = attn_decode_kv8_kernel<D, NT, FP8>;
-  const size_t smem = sizeof(DecodeKV8Smem<D, NT>);
-  static_assert(sizeof(DecodeKV8Smem<D, NT>) <= 113 * 1024, "two CTAs of an SM share its shared memory");
+  auto k = attn_decode_kv8_kernel<D, NT, CL, FP8>;
+  const size_t smem = sizeof(DecodeKV8Smem<D, NT, CL>);
+  static_assert(sizeof(DecodeKV8Smem<D, NT, CL>) <= 113 * 1024, "two CTAs of an SM share its shared memory");
   // The clusters that fit the device at once take equal runs; one more would start when the
   // others are done. (Groups of SMs that hold no whole number of clusters leave slots empty.)
   static std::atomic<int> fit[kKV8MaxDevices];
@@ -892,23 +909,38 @@ static cudaError_t launch_decode(AttnDecodeKV8Args a, cudaStream_t st) {
   if (n == 0) {
     e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = kKV8CL;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kKV8CL);
-    cfg.blockDim = dim3(kKV8Warps * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    e = cudaOccupancyMaxActiveClusters(&n, k, &cfg);
+    if (CL == 1) {
+      int per_sm = 0, sms = 0;
+      e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, kKV8Warps * 32, smem);
+      if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+      n = per_sm * sms;
+    } else {
+      cudaLaunchAttribute at;
+      at.id = cudaLaunchAttributeClusterDimension;
+      at.val.clusterDim.x = CL;
+      at.val.clusterDim.y = at.val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(CL);
+      cfg.blockDim = dim3(kKV8Warps * 32);
+      cfg.dynamicSmemBytes = smem;
+      cfg.attrs = &at;
+      cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&n, k, &cfg);
+    }
     if (e != cudaSuccess) return e;
-    n = n < 1 ? 1 : n;
+    n = n < 1 ? 1 : n > kKV8MaxCtas / CL ? kKV8MaxCtas / CL : n;
     fit[dev].store(n, std::memory_order_relaxed);
   }
-  a.clusters = n < a.clusters ? n : a.clusters;
-  return hx_launch_pdl_cluster(k, dim3((unsigned)(a.clusters * kKV8CL)), dim3(kKV8Warps * 32), smem, st, kKV8CL, a);
+  const dim3 grid((unsigned)(n * CL)), block(kKV8Warps * 32);
+  if (CL == 1) return hx_launch_pdl(k, grid, block, smem, st, a);
+  return hx_launch_pdl_cluster(k, grid, block, smem, st, CL, a);
+}
+
+template <int D, int NT, bool FP8>
+static cudaError_t launch_decode_cl(const AttnDecodeKV8Args& a, cudaStream_t st) {
+  // Few pairs: their blocks spread over many CTAs, whose partials four to a cluster merge on chip.
+  // From 12 on a pair's partials are few, and single CTAs save the cluster's barriers.
+  return a.B * a.c.Hkv * a.HG >= 12 ? launch_decode<D, NT, 1, FP8>(a, st) : launch_decode<D, NT, 4, FP8>(a, st);
 }
 
 cudaError_t attn_decode_kv8_launch(const AttnDecodeKV8Args& a, cudaStream_t st) {
@@ -917,9 +949,9 @@ cudaError_t attn_decode_kv8_launch(const AttnDecodeKV8Args& a, cudaStream_t st) 
     constexpr int D = decltype(d)::value;
     constexpr bool F = decltype(fp8)::value;
     if (a.NT == 1) {
-      e = launch_decode<D, 1, F>(a, st);
+      e = launch_decode_cl<D, 1, F>(a, st);
     } else if constexpr (D <= 128) {
-      e = launch_decode<D, 2, F>(a, st);
+      e = launch_decode_cl<D, 2, F>(a, st);
     } else {
       e = cudaErrorInvalidValue;
     }

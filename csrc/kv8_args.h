@@ -57,17 +57,16 @@ struct AttnDecodeKV8Args {
   int* ws;                    // word 0: errors; kKV8Err + pair: blocks done; kKV8PartAt: partials
   __nv_bfloat16* out;         // [B, Hq * D]
   int B, Hq, rot, gated;
-  int NT, HG;                 // query heads of a kv head: HG groups of at most 8 NT
-  int clusters;
+  int G, NT, HG, per;         // G query heads of a kv head: HG groups of per (at most 8 NT)
+  int vec;                    // rows of proj are 16-byte aligned
   float eps, sl2;             // scale * log2(e)
 };
 
-constexpr int kKV8CL = 4;           // CTAs of a decode cluster
 constexpr int kKV8Err = 64;         // words before the counters
 constexpr int kKV8MaxPairs = 16384; // (sequence, kv head, head group)s of a decode call
 constexpr int kKV8PartAt = kKV8Err + kKV8MaxPairs;  // the same for every batch that shares a scratch
 constexpr int kKV8MaxBatch = 256;   // sequences of a decode call
-constexpr int kKV8MaxPart = 80;     // most clusters, and so most partials of a pair
+constexpr int kKV8MaxCtas = 320;    // most CTAs of a decode launch, and so most partials of a pair
 
 // Query heads of one kv head are taken in groups of 8 or 16 (the tensor cores' columns); at
 // head dim 256 sixteen heads' sums do not fit a warp's registers.

@@ -115,16 +115,10 @@ void kv8_read(torch::Tensor kc, torch::Tensor vc, torch::Tensor ks, torch::Tenso
   HX_KV8_LAUNCH(kv8_read_launch(a, at::cuda::getCurrentCUDAStream()));
 }
 
-// Clusters of a decode launch: two CTAs fit an SM.
-static int kv8_clusters(c10::DeviceIndex dev) {
-  const int sms = at::cuda::getDeviceProperties(dev)->multiProcessorCount;
-  return std::min(kKV8MaxPart, 2 * sms / kKV8CL);
-}
-
 // Words of the scratch: (error, counters), then the partials' O, max and sum.
-static int64_t kv8_ws_words(int64_t clusters, int64_t pairs, int64_t D, int NT) {
+static int64_t kv8_ws_words(int64_t pairs, int64_t D, int NT) {
   TORCH_CHECK(pairs <= kKV8MaxPairs, "at most ", kKV8MaxPairs, " sequences x kv heads");
-  return kKV8PartAt + (clusters + pairs) * (8 * NT) * (D + 2);
+  return kKV8PartAt + (kKV8MaxCtas + pairs) * (8 * NT) * (D + 2);
 }
 
 // int32 scratch of attn_decode_kv8 for up to B sequences, zeroed; word 0 is its error word
@@ -136,9 +130,8 @@ torch::Tensor kv8_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
   TORCH_CHECK(D == 64 || D == 128 || D == 256, "head dim 64, 128 or 256");
   const int G = (int)(Hq / Hkv);
   const int64_t pairs = B * Hkv * kv8_groups(G, (int)D);
-  const auto dev = at::cuda::current_device();
-  return torch::zeros({kv8_ws_words(kv8_clusters(dev), pairs, D, kv8_tiles(G, (int)D))},
-                      torch::TensorOptions().dtype(torch::kInt).device(torch::kCUDA, dev));
+  return torch::zeros({kv8_ws_words(pairs, D, kv8_tiles(G, (int)D))},
+                      torch::TensorOptions().dtype(torch::kInt).device(torch::kCUDA, at::cuda::current_device()));
 }
 
 void attn_decode_kv8(torch::Tensor proj, c10::optional<torch::Tensor> q_norm_w, c10::optional<torch::Tensor> k_norm_w,
@@ -170,10 +163,12 @@ void attn_decode_kv8(torch::Tensor proj, c10::optional<torch::Tensor> q_norm_w, 
   TORCH_CHECK(B <= kKV8MaxBatch, "at most ", kKV8MaxBatch, " sequences");
   a.NT = kv8_tiles((int)(Hq / Hkv), (int)D);
   a.HG = kv8_groups((int)(Hq / Hkv), (int)D);
+  a.G = (int)(Hq / Hkv);
+  a.per = (a.G + a.HG - 1) / a.HG;
+  a.vec = reinterpret_cast<uintptr_t>(proj.data_ptr()) % 16 == 0 && (B <= 1 || proj.stride(0) % 8 == 0);
   TORCH_CHECK((double)B * Hkv * a.HG * a.c.nb < 2e9, "more than 2^31 blocks to attend to");
-  a.clusters = kv8_clusters(kc.device().index());
   TORCH_CHECK(ws.scalar_type() == at::kInt && ws.is_contiguous() &&
-                  ws.numel() >= kv8_ws_words(a.clusters, B * Hkv * a.HG, D, a.NT),
+                  ws.numel() >= kv8_ws_words(B * Hkv * a.HG, D, a.NT),
               "ws: from kv8_workspace() for as many sequences and heads");
   kv8_check_on(kc, proj, "proj");
   kv8_check_on(kc, inv_freq, "inv_freq");
