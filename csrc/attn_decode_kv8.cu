@@ -7,14 +7,13 @@
 // for codes c (K) and c' (V) of block b: the codes are exact in f16, so both products run on the
 // tensor cores over codes, and the scales are f32 factors outside them.
 //
-// Work is laid out as one list of blocks (32 keys of one sequence and kv head) over the whole
-// ragged batch. CTAs, or clusters of four, take equal runs of it, so sequences of any mix of lengths
-// load every SM alike; a run may end inside a pair (sequence, kv head) and go on into the next.
-// Inside a run's part of one pair (a segment) every warp of the cluster takes whole blocks, a
+// Every pair (sequence, kv head) of the ragged batch is cut into units of at most so many blocks of
+// 32 keys that the launch's CTAs, or clusters of four, take one unit each: the kernel finds the
+// fewest from the positions on the device. Inside a unit every warp takes whole blocks, a
 // warp with its own ring of bulk copies: K and V blocks are contiguous panels, so a copy is one
 // 2 or 4 KB piece and no warp waits for another. The warps' (max, sum, O) merge through shared
-// memory, the CTAs' through distributed shared memory, and segments of one pair through global
-// scratch, merged by the cluster that finishes last.
+// memory, the CTAs' through distributed shared memory, and units of one pair through global
+// scratch, merged by the one that finishes last.
 //
 // q and k stay in f32 between the norm, the rotation and the products; K is rounded to bf16
 // once, as it enters the cache. q enters the products in f16 after a power of two that brings
@@ -66,9 +65,9 @@ struct DecodeKV8Smem {
   float cm[GP], cl[GP];                  // this CTA's (max, sum)
   float lsum[GP];                        // the pair's sums in the last merge
   uint64_t full[kKV8Warps][KV8Ring<D>::kSlots];
-  int off[kKV8MaxBatch + 1];             // blocks before sequence b
-  int slot[kKV8MaxBatch], pos[kKV8MaxBatch];
-  int nbmax;
+  int off[kKV8MaxBatch + 1];             // units before sequence b
+  int slot[kKV8MaxBatch], pos[kKV8MaxBatch], nb[kKV8MaxBatch];  // its slot, position, blocks
+  int chunk;                             // most blocks of a unit
   uint32_t red[2][kKV8Warps];
   float inv[2], scale[2];
   int last;
@@ -275,30 +274,60 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
   }
   pdl_wait_prior();
   pdl_launch_dependents();
-  for (int d = tid; d < D; d += NTH) {
-    s->wq[d] = a.q_norm_w ? a.q_norm_w[d] : 1.f;
-    s->wk[d] = a.k_norm_w ? a.k_norm_w[d] : 1.f;
-  }
+  // ---- the list of units: a pair (sequence, kv head, head group) cut in equal parts -------------
+  // (every load that does not hang on another is issued first)
+  const int first = warp == 0 && lane < a.c.S ? a.pos[lane] : -1;  // of slots 0..31, beside the slot ids
+  const int slot0 = warp == 0 && lane < a.B ? a.slots[lane] : -1;
   const float freq = tid < a.rot / 2 ? a.inv_freq[tid] : 0.f;
   static_assert(D / 2 <= NTH, "a thread for each rotary frequency");
-  // ---- blocks of each sequence (0: refused), and the blocks before it -------------------------
+  constexpr int ND = (D + NTH - 1) / NTH;
+  float wq[ND], wk[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    const int d = i * NTH + tid;
+    wq[i] = a.q_norm_w && d < D ? a.q_norm_w[d] : 1.f;
+    wk[i] = a.k_norm_w && d < D ? a.k_norm_w[d] : 1.f;
+  }
   if (warp == 0) {
-    int base = 0, most = 0;
-    const int first = lane < a.c.S ? a.pos[lane] : -1;  // of slots 0..31, fetched with the slot ids
+    int sum = 0, most = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < a.B; b0 += 32) {
-      int n = 0;
-      const int slot = b0 + lane < a.B ? a.slots[b0 + lane] : -1;
+      const bool in = b0 + lane < a.B;
+      const int slot = b0 == 0 ? slot0 : in ? a.slots[b0 + lane] : -1;
       int p = __shfl_sync(0xffffffffu, first, slot & 31);
       if (slot < 0 || slot >= a.c.S) p = -1;
       else if (slot >= 32) p = a.pos[slot];
-      if (b0 + lane < a.B) {
-        n = p >= 0 && p < a.c.nb * kKV8Block ? p / kKV8Block + 1 : 0;
+      const int n = in && p >= 0 && p < a.c.nb * kKV8Block ? p / kKV8Block + 1 : 0;  // 0: refused
+      if (in) {
         s->slot[b0 + lane] = slot;
         s->pos[b0 + lane] = p;
+        s->nb[b0 + lane] = n;
       }
       most = max(most, n);
-      int x = n;
+      sum += n;
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    __syncwarp();
+    // Blocks of a unit: the fewest for which the launch holds all units at once, so that no CTA
+    // takes a second one; whole pairs where there are more pairs than that. Each lane tries one
+    // size between W / NC and the size that is enough for any mix of lengths.
+    const int W = sum * PB, pairs = a.B * PB;  // the host has checked that they fit
+    int chunk = most;
+    if (pairs < NC && most > 0) {
+      const int lo = (W + NC - 1) / NC, hi = (W + NC - pairs - 1) / (NC - pairs);
+      chunk = lo + (int)((long long)(hi - lo) * lane / 31);
+      int units = 0;
+#pragma unroll 1
+      for (int b = 0; b < a.B; ++b) units += (s->nb[b] + chunk - 1) / chunk;
+      chunk = __reduce_min_sync(0xffffffffu, units * PB <= NC || lane == 31 ? chunk : hi);
+    }
+    // at least a block for every warp where a pair has as many: more parts only add partials to merge
+    chunk = max(chunk, min(most, CL * NW));
+    int base = 0;
+#pragma unroll 1
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      int x = b0 + lane < a.B && chunk > 0 ? (s->nb[b0 + lane] + chunk - 1) / chunk * PB : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
@@ -307,46 +336,48 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       if (b0 + lane < a.B) s->off[b0 + lane + 1] = base + x;
       base += __shfl_sync(0xffffffffu, x, 31);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     if (lane == 0) {
       s->off[0] = 0;
-      s->nbmax = most;
+      s->chunk = chunk;
     }
   }
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+    if (i * NTH + tid < D) {
+      s->wq[i * NTH + tid] = wq[i];
+      s->wk[i * NTH + tid] = wk[i];
+    }
   __syncthreads();
-  if (cid == 0 && crank == 0)  // refused sequences: no cache access, a zero row, the error word
+  if (blockIdx.x == 0)  // refused sequences: no cache access, a zero row, the error word
+#pragma unroll 1
     for (int b = 0; b < a.B; ++b)
-      if (s->off[b + 1] == s->off[b]) {
+      if (s->nb[b] == 0) {
         for (int i = tid; i < a.Hq * D; i += NTH) a.out[(long long)b * a.Hq * D + i] = __float2bfloat16(0.f);
         if (tid == 0) atomicCAS(a.ws, 0, 6001);
       }
-  // Runs of `chunk` blocks. At least a block for every warp of the cluster where a pair has as
-  // many: a pair split further would only add partials to merge.
-  const int W = s->off[a.B] * PB;  // the host has checked that it fits
-  const int chunk = max((W + NC - 1) / NC, min(s->nbmax, CL * NW));
-  if ((long long)cid * chunk >= W) return;  // the whole cluster
-  int w = cid * chunk;
-  const int wend = min(W - w, chunk) + w;
-  float* part_o = reinterpret_cast<float*>(a.ws + kKV8PartAt);  // [NC + pairs][GP][D]
-  float2* part_ml = reinterpret_cast<float2*>(part_o + (long long)(NC + a.B * PB) * GP * D);  // [NC + pairs][GP]
+  const int units = s->off[a.B];
+  float* part_o = reinterpret_cast<float*>(a.ws + kKV8PartAt);  // [units][GP][D]
+  float2* part_ml = reinterpret_cast<float2*>(part_o + (long long)(kKV8MaxCtas + a.B * PB) * GP * D);  // [units][GP]
   int put = 0, get = 0;  // ring slots of the next copy issued (lane 0) and used
   uint32_t phase = 0;    // parity of the slot to use next
   bool ok = true;
   DecodeKV8Warp<D, NT, FP8> st;
-  int b = 0;
-  for (int lo = 0, hi = a.B; lo < hi;) {  // the sequence of the run's first block
-    b = (lo + hi) / 2;
-    if (s->off[b + 1] * PB <= w) lo = b + 1;
-    else hi = b;
-    b = lo;
-  }
-  while (w < wend) {
-    while (s->off[b + 1] * PB <= w) ++b;
-    const int nb = s->off[b + 1] - s->off[b];
-    const int pl = (w - s->off[b] * PB) / nb;  // kv head and head group
-    const int p0 = s->off[b] * PB + pl * nb;   // the pair's first block in the list
-    const int blk0 = w - p0, blk1 = min(nb, wend - p0);
+#pragma unroll 1
+  for (int unit = cid; unit < units; unit += NC) {
+    int b = 0;  // its sequence
+#pragma unroll 1
+    for (int hi = a.B - 1; b < hi;) {
+      const int mid = (b + hi) / 2;
+      if (s->off[mid + 1] <= unit) b = mid + 1;
+      else hi = mid;
+    }
+    const int nb = s->nb[b], cuts = (nb + s->chunk - 1) / s->chunk;  // parts of each of its pairs
+    const int pl = (unit - s->off[b]) / cuts, part = unit - s->off[b] - pl * cuts;
+    const int u0 = unit - part;  // the pair's first unit
+    // The part with the last block has more to do there; it gets fewer of the others.
+    const int heavy = cuts > 1 ? min(12, s->chunk / 4) : 0;
+    const int blk0 = (int)((long long)part * (nb + heavy) / cuts);
+    const int blk1 = part + 1 == cuts ? nb : (int)((long long)(part + 1) * (nb + heavy) / cuts);
     const int pair = b * PB + pl, h = HG == 1 ? pl : pl / HG, hg = pl - h * HG, g0 = hg * per, n = min(per, G - g0);
     const int slot = s->slot[b], p = s->pos[b], row = p % kKV8Block;
     const __nv_bfloat16* pr = a.proj + b * a.ldp;
@@ -378,8 +409,19 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
 #pragma unroll 1
       for (int i = 0; i < R::kSlots && todo > 0 && ok && lane == 0; ++i) issue();
     };
-    if (!(completes && warp == host)) fill();
-    // ---- loads that the segment's start needs, in flight together --------------------------------
+    // ---- loads that the unit's start needs, ahead of the copies --------------------------------
+    constexpr int LR = D / 8, RP = NTH / LR, PS = (GP + RP) / RP;  // lanes of a row of q, rows of a pass, passes
+    const int nrow = n + (cta_last ? 1 : 0);  // the group's queries, then the new key
+    const int rr = tid / LR, d0 = tid % LR * 8;
+    uint4 qx[PS], vx = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < PS; ++i) {
+      const int r = i * RP + rr;
+      const __nv_bfloat16* src = r == n ? pr + a.Hq * qw + h * D : pr + (long long)(h * G + g0 + r) * qw;
+      qx[i] = r < nrow ? load8_raw(src, d0, a.vec) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (cta_last && rr == 0) vx = load8_raw(pr + a.Hq * qw + (Hkv + h) * D, d0, a.vec);
+    const int delta = a.rope_delta ? a.rope_delta[slot] : 0;
     // The last block's bf16 rows, for the whole CTA: for a completed block 16-value pieces of the
     // block's layout (X[i][0..1] of K, [2..3] of V); else operands: warp w takes dims groups
     // (of 16) w * NP + i of the sums and of the output.
@@ -408,24 +450,21 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         }
       }
     }
+    if (!(completes && warp == host)) fill();
     // ---- q of the group's heads (and the new key): norm, rotation ------------------------------
-    // Rows go over D / 8 lanes each, 8 dims to a lane, in small loops: code that runs once a launch
-    // costs its fetch.
-    constexpr int LR = D / 8, RP = NTH / LR;  // lanes of a row, rows of a pass
-    const int nrow = n + (cta_last ? 1 : 0);  // the group's queries, then the new key
-    const int rr = tid / LR, d0 = tid % LR * 8;
+    // Rows go over D / 8 lanes each, 8 dims to a lane.
     auto row_max = [](auto x) {
 #pragma unroll
       for (int o = 1; o < LR; o <<= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
       return x;
     };
-#pragma unroll 1
-    for (int r = rr; r - rr < nrow; r += RP) {
+#pragma unroll
+    for (int i = 0; i < PS; ++i) {
+      const int r = i * RP + rr;
+      if (i * RP >= nrow) break;
       const bool isk = r == n;
-      const __nv_bfloat16* src = isk ? pr + a.Hq * qw + h * D : pr + (long long)(h * G + g0 + r) * qw;
-      const uint4 x = r < nrow ? load8_raw(src, d0, a.vec) : make_uint4(0u, 0u, 0u, 0u);
       float f[8];
-      unpack8(*reinterpret_cast<const bf16x8*>(&x), f);
+      unpack8(*reinterpret_cast<const bf16x8*>(&qx[i]), f);
       if (a.q_norm_w || a.k_norm_w) {  // (weights of an absent norm are 1, its factor too)
         float ss = 0.f;
 #pragma unroll
@@ -443,12 +482,10 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         dst[1] = make_float4(f[4], f[5], f[6], f[7]);
       }
     }
-    if (cta_last && rr == 0)
-      *reinterpret_cast<uint4*>(s->vnew + d0) = load8_raw(pr + a.Hq * qw + (Hkv + h) * D, d0, a.vec);
+    if (cta_last && rr == 0) *reinterpret_cast<uint4*>(s->vnew + d0) = vx;
     const int half = a.rot / 2;
     if (half) {
-      const int prot = p + (a.rope_delta ? a.rope_delta[slot] : 0);
-      if (tid < half) rotation((float)prot * freq, &s->sn[tid], &s->cs[tid]);
+      if (tid < half) rotation((float)(p + delta) * freq, &s->sn[tid], &s->cs[tid]);
       __syncthreads();
 #pragma unroll 1
       for (int r = warp; r < nrow; r += NW) {
@@ -802,7 +839,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       y.y = pack_bf16x2(f[2], f[3]);
       *reinterpret_cast<uint2*>(a.out + ((long long)b * a.Hq + hq) * D + d) = y;
     };
-    const bool alone = blk0 == 0 && blk1 == nb;
+    const bool alone = cuts == 1;
     const int cols = n * (D / 4) / CL, c0 = crank * cols;  // in fours
 #pragma unroll 1
     for (int i = c0 + tid; i < c0 + cols; i += NTH) {
@@ -826,18 +863,18 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       if (alone) {
         finish(r, d, O, L);
       } else {
-        reinterpret_cast<float4*>(part_o + (long long)(cid + pair) * (GP * D))[i] = O;
-        if (d == 0) part_ml[(long long)(cid + pair) * GP + r] = make_float2(M, L);
+        reinterpret_cast<float4*>(part_o + (long long)unit * (GP * D))[i] = O;
+        if (d == 0) part_ml[(long long)unit * GP + r] = make_float2(M, L);
       }
     }
     if (!alone) __threadfence();
-    tc::fence_proxy_async_smem();  // O's stores before the next segment's copies into the same memory
+    tc::fence_proxy_async_smem();  // O's stores before the next unit's copies into the same memory
     all_sync();
     if (!alone) {
-      // the cluster that completes the pair's block count merges its partials
+      // the CTA or cluster that finishes the last of the pair's units merges their partials
       if (crank == 0 && tid == 0) {
         int* counter = a.ws + kKV8Err + pair;
-        const int last = atomicAdd(counter, blk1 - blk0) + (blk1 - blk0) == nb;
+        const int last = atomicAdd(counter, 1) == cuts - 1;
         if (last) *counter = 0;
         __threadfence();
         for (int x = 0; x < CL; ++x) *peer(&s->last, x) = last;
@@ -845,8 +882,8 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       all_sync();
       if (s->last) {
         __threadfence();
-        const int f0 = p0 / chunk, np = (p0 + nb - 1) / chunk - f0 + 1;  // its clusters
-        const long long q0 = f0 + pair;
+        const int np = cuts;
+        const long long q0 = u0;
         const int r0 = c0 / (D / 4), r1 = (c0 + cols - 1) / (D / 4);       // heads of this CTA's columns
 #pragma unroll 1
         for (int r = r0 + warp; r <= r1; r += NW) {
@@ -889,7 +926,6 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         __syncthreads();
       }
     }
-    w = p0 + blk1;
   }
 }
 

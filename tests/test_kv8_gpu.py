@@ -198,6 +198,9 @@ DECODE = [
     (256, 2, 8, True, 64, [1900, 700]),
     (256, 1, 5, False, 256, [30, 31, 0]),
     (256, 1, 16, True, 64, [330, 31]),
+    # more pairs than CTAs: each takes several units; and one long sequence among empty ones
+    (64, 8, 2, False, 64, [(i * 37) % 90 for i in range(48)]),
+    (128, 2, 4, False, 128, [0] * 9 + [6001] + [1] * 30),
 ]
 
 
