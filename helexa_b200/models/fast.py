@@ -9,6 +9,7 @@ any subset of live sequences without the reference's assemble/extract copies
   kc, vc    bf16  [S, Hkv, maxlen, D] per full-attention layer (contiguous, never
                                       re-concatenated -- the ref's ConcatKvCache
                                       reallocates on every append, full_attn.rs:156)
+            or, with kv_dtype "int8" / "fp8", an 8-bit cache per layer (ops/kv8.py)
   conv      bf16  [S, C, K]           GDN conv inputs, ring indexed by position % K
   rec       f32   [S, Hv, Dk, Dv]     GDN recurrent state
 
@@ -28,6 +29,7 @@ import torch
 
 from .. import ops
 from ..config import ModelConfig
+from ..ops.kv8 import KV8
 from . import layout
 
 
@@ -87,6 +89,7 @@ class DecodeBuffers:
     sgraph_steps: int = 0
     logits_full: torch.Tensor | None = None       # f32 [B, V] (vocab-parallel gather target)
     _gather_buf: torch.Tensor | None = None
+    kv8_ws: torch.Tensor | None = None            # int32 scratch of attn_decode_kv8 (word 0: errors)
 
 
 class SamplerState:
@@ -158,7 +161,12 @@ class DeviceError(RuntimeError):
     peer never arrived; other codes: a GEMM pipeline wait)."""
 
     def __init__(self, code: int):
-        what = f"tensor-parallel peer {code % 1000} never arrived" if code >= 1000 else "GEMM pipeline wait ran out"
+        if code == 6001:
+            what = "a slot or position outside the 8-bit KV cache"
+        elif code == 6002 or 7000 < code < 8000:
+            what = "8-bit KV attention wait ran out"
+        else:
+            what = f"tensor-parallel peer {code % 1000} never arrived" if code >= 1000 else "GEMM pipeline wait ran out"
         super().__init__(f"device error {code}: {what}")
         self.code = code
 
@@ -266,11 +274,16 @@ class FastModel:
     def __init__(self, cfg: ModelConfig, layers: list[dict[str, torch.Tensor]], embed: torch.Tensor,
                  lm_head: torch.Tensor, final_norm: torch.Tensor, dims: layout.LocalDims,
                  device: torch.device, max_slots: int = 4, max_len: int = 16384, comm=None,
-                 attn_splits: int | None = None):
+                 attn_splits: int | None = None, kv_dtype: str = "bf16"):
         if device.type != "cuda" and not _allow_cpu_prefill:
             raise ValueError("FastModel runs on CUDA only; use ReferenceModel on the CPU")
         self.cfg, self.dims, self.device = cfg, dims, device
         self.layers, self.embed_w, self.lm_head, self.final_norm = layers, embed, lm_head, final_norm
+        if kv_dtype not in ("bf16", "int8", "fp8"):
+            raise ValueError(f"unknown kv_dtype {kv_dtype!r}; one of bf16, int8, fp8")
+        if kv_dtype != "bf16" and device.type != "cuda":
+            raise ValueError("the 8-bit KV cache runs on CUDA only")
+        self.kv_dtype = kv_dtype
         self.max_slots, self.max_len = max_slots, max_len
         self._xscratch = None  # bf16 scratch for dequantized expert stacks (prefill)
         self.comm = comm  # parallel.TPComm or None (single rank)
@@ -297,6 +310,7 @@ class FastModel:
         self.pos = torch.zeros(max_slots, dtype=torch.int32, device=device)
         self.kc: dict[int, torch.Tensor] = {}
         self.vc: dict[int, torch.Tensor] = {}
+        self.kv8: dict[int, KV8] = {}
         self.conv: dict[int, torch.Tensor] = {}
         self.rec: dict[int, torch.Tensor] = {}
         for i in range(cfg.num_hidden_layers):
@@ -305,6 +319,8 @@ class FastModel:
                                            dtype=torch.bfloat16, device=device)
                 self.rec[i] = torch.zeros(max_slots, dims.hv, dims.dk, dims.dv, dtype=torch.float32,
                                           device=device)
+            elif kv_dtype != "bf16":
+                self.kv8[i] = KV8.alloc(max_slots, dims.hkv, max_len, dims.D, kv_dtype, device)
             else:
                 shp = (max_slots, dims.hkv, max_len, dims.D)
                 self.kc[i] = torch.zeros(shp, dtype=torch.bfloat16, device=device)
@@ -464,6 +480,7 @@ class FastModel:
         bf, f32, i32 = torch.bfloat16, torch.float32, torch.int32
         z = lambda *s, dt=bf: torch.zeros(*s, dtype=dt, device=dev)  # noqa: E731
         J = cfg.num_experts_per_tok + (1 if self.has_shared else 0)
+        split = cfg.num_full_layers and not self.kv8  # bf16 attention's split-K scratch
         any_mlp = any(not cfg.layer_uses_moe(i) for i in range(cfg.num_hidden_layers))
         nb = DecodeBuffers(
             B=B, tok=z(B, dt=i32), slots=torch.arange(B, dtype=i32, device=dev), x=z(B, d.H),
@@ -471,9 +488,9 @@ class FastModel:
             gdn_out=z(B, d.gdn_vd) if cfg.num_linear_layers else None,
             proj_attn=z(B, d.qkv_rows) if cfg.num_full_layers else None,
             attn_out=z(B, d.hq * d.D) if cfg.num_full_layers else None,
-            part_o=z(B, d.hq, self._splits_for(B), d.D, dt=f32) if cfg.num_full_layers else None,
-            part_ml=z(B, d.hq, self._splits_for(B), 2, dt=f32) if cfg.num_full_layers else None,
-            counters=z(B, max(1, d.hkv), dt=i32) if cfg.num_full_layers else None,
+            part_o=z(B, d.hq, self._splits_for(B), d.D, dt=f32) if split else None,
+            part_ml=z(B, d.hq, self._splits_for(B), 2, dt=f32) if split else None,
+            counters=z(B, max(1, d.hkv), dt=i32) if split else None,
             rlogits=z(B, cfg.num_experts + (1 if self.has_shared else 0), dt=f32) if cfg.num_experts else None,
             ids=z(B, J, dt=i32) if cfg.num_experts else None,
             wts=z(B, J, dt=f32) if cfg.num_experts else None,
@@ -482,6 +499,8 @@ class FastModel:
             partial=z(B, d.H),
             logits=z(B, self.v_local, dt=f32), out_tokens=z(B, out_cap, dt=i32), step=z(B, dt=i32),
             best=z(B, dt=torch.int64), counter=z(1, dt=i32), err=z(1, dt=i32))
+        if self.kv8:
+            nb.kv8_ws = self.C.kv8_workspace(B, d.hq, d.hkv, d.D)
         self._bufs[B] = nb
         return nb
 
@@ -531,9 +550,15 @@ class FastModel:
             self._row_parallel(lw["out_w"], nb.gdn_out, nb)
         else:
             self._gemv(lw["w_qkv"], nb.x, nb.proj_attn, ops.STORE_BF16, None, lw["ln1"], eps)
-            C.attn_decode(nb.proj_attn, lw.get("q_norm"), lw.get("k_norm"), self.inv_freq, self.kc[i], self.vc[i],
-                          nb.slots, self.pos, nb.part_o, nb.part_ml, nb.counters, nb.attn_out, d.hq, d.hkv, d.D,
-                          cfg.rotary_dim, cfg.attn_output_gate, eps, self.rope_delta if self.mrope else None)
+            delta = self.rope_delta if self.mrope else None
+            if self.kv8:
+                C.attn_decode_kv8(nb.proj_attn, lw.get("q_norm"), lw.get("k_norm"), self.inv_freq, *self.kv8[i],
+                                  nb.slots, self.pos, nb.kv8_ws, nb.attn_out, d.hq, cfg.rotary_dim,
+                                  cfg.attn_output_gate, eps, delta)
+            else:
+                C.attn_decode(nb.proj_attn, lw.get("q_norm"), lw.get("k_norm"), self.inv_freq, self.kc[i],
+                              self.vc[i], nb.slots, self.pos, nb.part_o, nb.part_ml, nb.counters, nb.attn_out, d.hq,
+                              d.hkv, d.D, cfg.rotary_dim, cfg.attn_output_gate, eps, delta)
             self._row_parallel(lw["o_w"], nb.attn_out, nb)
         if cfg.layer_uses_moe(i):
             E, k = cfg.num_experts, cfg.num_experts_per_tok
@@ -715,7 +740,7 @@ class FastModel:
         n = 3  # embedding, first norm, lm_head GEMM of the last token
         for i in range(cfg.num_hidden_layers):
             # in_proj, prep, chunk, scan, onorm, out, conv ring | qkv, q/k-norm+rope+KV, attn, o
-            n += 5 + 3 if cfg.is_linear(i) else 4
+            n += 5 + 3 if cfg.is_linear(i) else 4 + (1 if self.kv8 else 0)  # 8-bit: the append is its own
             n += 7 if cfg.layer_uses_moe(i) else 2          # router, topk, plan, place, 2 grouped, combine | 2 GEMMs
             n += 2                                          # two fused (reduce +) residual + norm kernels
         return n
@@ -841,7 +866,7 @@ class FastModel:
     def device_error(self) -> int:
         """First nonzero device error word (GEMM bounded waits, TP exchange), else 0.
         Reading it synchronizes the device."""
-        words = [self._gemm_err()]
+        words = [self._gemm_err()] + [nb.kv8_ws for nb in self._bufs.values() if nb.kv8_ws is not None]
         if self.comm is not None and getattr(self.comm, "err", None) is not None:
             words.append(self.comm.err)
         for v in torch.cat([w.view(-1)[:1] for w in words]).tolist():
@@ -957,13 +982,23 @@ class FastModel:
             # gate is applied in the attention kernel's epilogue
             q = torch.empty(T, d.hq * D, dtype=torch.bfloat16, device=h.device)
             pos3 = self._pos3
+            if self.kv8:  # the chunk's own K / V rows, at positions p0 .. by the rotary offset
+                kc, vc = torch.empty(2, d.hkv, T, D, dtype=torch.bfloat16, device=h.device)
+                at, off = 0, p0
+            else:
+                kc, vc, at, off = self.kc[i][slot], self.vc[i][slot], p0, 0
             self.C.qk_rope_kv(qkv, d.hq, d.hkv, D, d.qw, lw.get("q_norm"), lw.get("k_norm"), self.inv_freq,
-                              cfg.rotary_dim, self.kc[i][slot], self.vc[i][slot], p0, q, cfg.rms_norm_eps,
-                              pos3, self.mrope_axes if pos3 is not None else None, self._rope_delta_host[slot])
+                              cfg.rotary_dim, kc, vc, at, q, cfg.rms_norm_eps,
+                              pos3, self.mrope_axes if pos3 is not None else None,
+                              off + self._rope_delta_host[slot])
             o = torch.empty(T, d.hq * D, dtype=torch.bfloat16, device=h.device)
             gate = qkv[:, D:] if cfg.attn_output_gate else None
+            if self.kv8:
+                self.C.kv8_append(kc.transpose(0, 1), vc.transpose(0, 1), *self.kv8[i], slot, p0)
             self._mark("attn.core")
-            if self.attn_engine == "tc":
+            if self.kv8:
+                self.C.attn_prefill_kv8(q, *self.kv8[i], slot, p0, o, d.hq, D ** -0.5, gate, d.qw, self._gemm_err())
+            elif self.attn_engine == "tc":
                 self.C.attn_prefill_tc(q, self.kc[i][slot], self.vc[i][slot], o, d.hq, p0, D ** -0.5, gate, d.qw,
                                        self._gemm_err())
             else:

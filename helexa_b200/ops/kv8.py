@@ -1,0 +1,87 @@
+"""The 8-bit KV cache of one attention layer (csrc/kv8.cuh has the layout and the codes).
+
+Tokens are held in blocks of 32. A complete block has int8 or float8_e4m3 codes and one f32
+scale for each kv head, for K and for V; the sequence's last block is also kept in bf16 (the
+tail) and is read from there until it is complete. So the cache holds the same bytes however
+its tokens arrived, at (D + 1/8) bytes a token and head instead of 2 D.
+
+    cache = KV8.alloc(slots, hkv, max_len, head_dim, "int8", "cuda")
+    ops.C.kv8_append(k, v, *cache, slot, p0)             # k, v [T, Hkv, D] bf16
+    k, v = cache.read(slot, length)                      # bf16 [Hkv, length, D]
+    ws = ops.C.kv8_workspace(B, Hq, hkv, head_dim)       # one for each stream that decodes
+    ops.C.attn_decode_kv8(proj, qn, kn, inv_freq, *cache, slots, pos, ws, out, Hq, rot, gated, eps)
+    ops.C.attn_prefill_kv8(q, *cache, slot, p0, out, Hq, scale, gate, gate_head_stride, err)
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+BLOCK = 32
+DTYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
+
+
+def bytes_per_token(hkv: int, head_dim: int) -> float:
+    """K + V codes and scales of one token in one layer."""
+    return 2 * hkv * (head_dim + 4 / BLOCK)
+
+
+def tail_bytes(hkv: int, head_dim: int) -> int:
+    """The bf16 copy of one slot's last block, K and V, in one layer."""
+    return 2 * hkv * BLOCK * head_dim * 2
+
+
+class KV8(NamedTuple):
+    kc: torch.Tensor   # [S, Hkv, NB, D/64, 32, 64] codes of K
+    vc: torch.Tensor   # [S, Hkv, NB, D/64, 64, 32] codes of V, keys innermost
+    ks: torch.Tensor   # f32 [S, Hkv, NB]
+    vs: torch.Tensor
+    kt: torch.Tensor   # bf16 [S, Hkv, D/64, 32, 64] the last block
+    vt: torch.Tensor   # bf16 [S, Hkv, D/64, 64, 32]
+
+    @classmethod
+    def alloc(cls, slots: int, hkv: int, max_len: int, head_dim: int, dtype: str, device) -> "KV8":
+        if dtype not in DTYPES:
+            raise ValueError(f"unknown 8-bit KV cache type {dtype!r}; one of {sorted(DTYPES)}")
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"the 8-bit KV cache needs head dim 64, 128 or 256, not {head_dim}")
+        nb, n = (max_len + BLOCK - 1) // BLOCK, head_dim // 64
+        z = lambda *s, dt: torch.zeros(slots, hkv, *s, dtype=dt, device=device)  # noqa: E731
+        bf, f32, c = torch.bfloat16, torch.float32, DTYPES[dtype]
+        return cls(z(nb, n, BLOCK, 64, dt=c), z(nb, n, 64, BLOCK, dt=c), z(nb, dt=f32), z(nb, dt=f32),
+                   z(n, BLOCK, 64, dt=bf), z(n, 64, BLOCK, dt=bf))
+
+    @property
+    def head_dim(self) -> int:
+        return self.kc.shape[3] * 64
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in self)
+
+    def read(self, slot: int, length: int, start: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+        """Rows start .. length-1 of a slot that holds `length` tokens, as bf16 [Hkv, n, D]."""
+        from . import C
+        k = torch.empty(self.kc.shape[1], length - start, self.head_dim, dtype=torch.bfloat16, device=self.kc.device)
+        v = torch.empty_like(k)
+        C.kv8_read(*self, slot, length, start, k, v)
+        return k, v
+
+    def snapshot(self, slot: int, length: int, held: int) -> tuple[torch.Tensor, ...]:
+        """Copies of what a continuation after `length` of the slot's `held` tokens needs. A cut
+        inside a block needs that block's bf16 rows, which only the last block has."""
+        if not 0 <= length <= held:
+            raise ValueError(f"a cut at {length} of {held} tokens")
+        if length % BLOCK and length // BLOCK != (held - 1) // BLOCK:
+            raise ValueError(f"an 8-bit cache of {held} tokens can be cut at whole blocks of {BLOCK} or inside "
+                             f"the last one, not at {length}")
+        n = length // BLOCK
+        # a block complete in the tail but cut inside is not read from its codes
+        return tuple(t[slot, :, :n].clone() for t in self[:4]) + tuple(t[slot].clone() for t in self[4:])
+
+    def restore(self, slot: int, saved: tuple[torch.Tensor, ...]) -> None:
+        n = saved[0].shape[1]
+        for t, s in zip(self[:4], saved[:4]):
+            t[slot, :, :n] = s
+        for t, s in zip(self[4:], saved[4:]):
+            t[slot] = s

@@ -9,9 +9,11 @@ controller's KV budget and each request's reservation.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 from ..config import ModelConfig
+from ..ops import kv8
 
 
 @dataclass
@@ -21,11 +23,14 @@ class ContextProfile:
     max_position: int
 
     @classmethod
-    def from_config(cls, cfg: ModelConfig, tp: int = 1) -> "ContextProfile":
+    def from_config(cls, cfg: ModelConfig, tp: int = 1, kv_dtype: str = "bf16") -> "ContextProfile":
         kv_heads_per_rank = max(1, cfg.num_key_value_heads // tp)
         kv = 2 * cfg.num_full_layers * kv_heads_per_rank * cfg.head_dim * 2
-        return cls(kv_bytes_per_token=kv, state_bytes_per_seq=cfg.gdn_state_bytes() // max(1, tp),
-                   max_position=cfg.max_position_embeddings)
+        state = cfg.gdn_state_bytes() // max(1, tp)
+        if kv_dtype != "bf16":  # 8-bit codes and scales; each slot's last block in bf16 as well
+            kv = math.ceil(cfg.num_full_layers * kv8.bytes_per_token(kv_heads_per_rank, cfg.head_dim))
+            state += cfg.num_full_layers * kv8.tail_bytes(kv_heads_per_rank, cfg.head_dim)
+        return cls(kv_bytes_per_token=kv, state_bytes_per_seq=state, max_position=cfg.max_position_embeddings)
 
 
 @dataclass

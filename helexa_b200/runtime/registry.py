@@ -34,6 +34,7 @@ class ModelSpec:
     source: str
     harness: str = "helexa"
     quant: str | None = None
+    kv_dtype: str = "bf16"          # KV cache: "bf16", or 8-bit "int8" / "fp8" (ops/kv8.py)
     tensor_parallel: int = 1
     devices: list[int] | None = None
     max_len: int = 16384
@@ -72,11 +73,23 @@ def free_device_bytes(dev: int) -> int:
     return free + max(0, torch.cuda.memory_reserved(dev) - torch.cuda.memory_allocated(dev))
 
 
+def check_kv_dtype(kv_dtype: str, cfg, use_cuda: bool) -> None:
+    if kv_dtype == "bf16":
+        return
+    if kv_dtype not in ("int8", "fp8"):
+        raise LoadError(f"unknown kv_dtype {kv_dtype!r}", "bad_kv_dtype", "one of bf16, int8, fp8")
+    if not use_cuda:
+        raise LoadError("the 8-bit KV cache needs a CUDA device", "bad_kv_dtype", "use kv_dtype bf16")
+    if cfg is not None and cfg.num_full_layers and cfg.head_dim not in (64, 128, 256):
+        raise LoadError(f"the 8-bit KV cache needs head dim 64, 128 or 256, not {cfg.head_dim}", "bad_kv_dtype",
+                        "use kv_dtype bf16")
+
+
 def plan_max_len(cfg, spec: "ModelSpec", free_bytes: int, weight_bytes: int) -> int:
     """KV length per slot that fits the tightest device after the weights, for the
     spec's slot count (context_limit.rs: free memory -> context)."""
     tp = max(1, spec.tensor_parallel)
-    prof = ContextProfile.from_config(cfg, tp)
+    prof = ContextProfile.from_config(cfg, tp, spec.kv_dtype)
     lim = derive_limit(prof, max(0, free_bytes - weight_bytes), floor_bytes=FLOOR_BYTES,
                        concurrent=spec.max_batch + 1)
     return max(0, min(spec.max_len, cfg.max_position_embeddings, lim.context))
@@ -86,6 +99,7 @@ def build_served_model(spec: ModelSpec) -> ServedModel:
     src = resolve_source(spec.source)
     cfg = src.config
     use_cuda = (spec.device or ("cuda" if torch.cuda.is_available() else "cpu")) == "cuda"
+    check_kv_dtype(spec.kv_dtype, cfg, use_cuda)
     devs_free = None
     if use_cuda:
         ids = spec.devices or list(range(spec.tensor_parallel))
@@ -113,7 +127,7 @@ def build_served_model(spec: ModelSpec) -> ServedModel:
                             "lower max_batch or use more tensor-parallel ranks")
         from ..models.fast import FastModel
         dev = torch.device("cuda", (spec.devices or [0])[0])
-        kw = dict(max_slots=spec.max_batch + 1, max_len=max_len)
+        kw = dict(max_slots=spec.max_batch + 1, max_len=max_len, kv_dtype=spec.kv_dtype)
         if src.kind == "preset":
             model = FastModel.random(cfg, dev, **kw)
         elif src.kind == "gguf":
@@ -127,7 +141,8 @@ def build_served_model(spec: ModelSpec) -> ServedModel:
         if spec.quant:  # in-situ quantization of the dense projections (ISQ)
             model.quantize_(spec.quant.upper())
         runner = FastRunner(model)
-        kv_bpt = cfg.kv_bytes_per_token()
+        kv_bpt = cfg.kv_bytes_per_token() if spec.kv_dtype == "bf16" else \
+            ContextProfile.from_config(cfg, 1, spec.kv_dtype).kv_bytes_per_token
         vget = None
         if cfg.vision and src.kind == "preset":
             from ..models.vision import VisionConfig, random_vision_weights

@@ -16,7 +16,7 @@ import torch
 @dataclass
 class Snapshot:
     length: int
-    kv: dict = field(default_factory=dict)     # layer -> (k [Hkv, L, D], v [Hkv, L, D])
+    kv: dict = field(default_factory=dict)     # layer -> (k [Hkv, L, D], v [Hkv, L, D]) or an 8-bit cache's parts
     conv: dict = field(default_factory=dict)   # layer -> ring / conv state
     rec: dict = field(default_factory=dict)    # layer -> recurrent state
     ref_state: object = None                   # CPU reference model state
@@ -25,8 +25,8 @@ class Snapshot:
     @property
     def nbytes(self) -> int:
         n = 0
-        for k, v in self.kv.values():
-            n += k.numel() * k.element_size() + v.numel() * v.element_size()
+        for parts in self.kv.values():
+            n += sum(t.numel() * t.element_size() for t in parts)
         for d in (self.conv, self.rec):
             for t in d.values():
                 n += t.numel() * t.element_size()
@@ -159,6 +159,8 @@ class FastRunner:
         snap = Snapshot(length=length)
         for i in m.kc:
             snap.kv[i] = (m.kc[i][slot, :, :length].clone(), m.vc[i][slot, :, :length].clone())
+        for i, c in m.kv8.items():
+            snap.kv[i] = c.snapshot(slot, length, self.host_pos[slot])
         for i in m.conv:
             snap.conv[i] = m.conv[i][slot].clone()
             snap.rec[i] = m.rec[i][slot].clone()
@@ -168,9 +170,11 @@ class FastRunner:
     def restore(self, slot: int, snap: Snapshot):
         m = self.m
         L = snap.length
-        for i, (k, v) in snap.kv.items():
-            m.kc[i][slot, :, :L] = k
-            m.vc[i][slot, :, :L] = v
+        for i, parts in snap.kv.items():
+            if i in m.kv8:
+                m.kv8[i].restore(slot, parts)
+                continue
+            m.kc[i][slot, :, :L], m.vc[i][slot, :, :L] = parts
         for i in snap.conv:
             m.conv[i][slot] = snap.conv[i]
             m.rec[i][slot] = snap.rec[i]

@@ -78,7 +78,8 @@ def cuda_fast_runner(rank: int, ws: int, cfg_args: dict):
     src = resolve_source(cfg_args["source"])
     cfg = src.config
     comm = TPComm(dist.group.WORLD, dev)
-    kw = dict(rank=rank, ws=ws, max_slots=cfg_args["max_slots"], max_len=cfg_args["max_len"], comm=comm)
+    kw = dict(rank=rank, ws=ws, max_slots=cfg_args["max_slots"], max_len=cfg_args["max_len"], comm=comm,
+              kv_dtype=cfg_args.get("kv_dtype", "bf16"))
     if src.kind == "preset":
         model = FastModel.random(cfg, dev, seed=0, **kw)
     elif src.kind == "gguf":
@@ -365,7 +366,7 @@ def build_tp_served_model(spec, src, cfg, devs_free: list[int]):
         raise LoadError(f"only {max_len} tokens of KV fit beside the weights", "insufficient_memory")
     runner = spawn_pool(tp, "helexa_b200.runtime.tp_pool:cuda_fast_runner",
                         {"source": spec.source, "max_slots": spec.max_batch + 1, "max_len": max_len,
-                         "quant": spec.quant}, devices=devices)
+                         "quant": spec.quant, "kv_dtype": spec.kv_dtype}, devices=devices)
     return serve_runner(spec, src, cfg, runner, devices, max_len)
 
 
@@ -374,6 +375,7 @@ def serve_runner(spec, src, cfg, runner, devices, max_len):
     from dataclasses import asdict
 
     from .admission import AdmissionConfig, AdmissionController
+    from .context_limit import ContextProfile
     from .engine import Engine
     from .prefix_cache import PrefixCache
     from .sampling import GenerationDefaults
@@ -387,7 +389,9 @@ def serve_runner(spec, src, cfg, runner, devices, max_len):
     adm = AdmissionController(AdmissionConfig(max_in_flight=spec.max_in_flight or spec.max_batch,
                                               max_queue_depth=spec.max_queue_depth, max_wait_s=spec.max_wait_s,
                                               max_per_principal=spec.max_per_principal))
-    kv_bpt = cfg.kv_bytes_per_token() // max(1, min(spec.tensor_parallel, cfg.num_key_value_heads or 1))
+    kv_ranks = max(1, min(spec.tensor_parallel, cfg.num_key_value_heads or 1))
+    kv_bpt = cfg.kv_bytes_per_token() // kv_ranks if spec.kv_dtype == "bf16" else \
+        ContextProfile.from_config(cfg, kv_ranks, spec.kv_dtype).kv_bytes_per_token
     adm.set_kv_budget_mb((kv_bpt * max_len * spec.max_batch) >> 20)
     defaults = GenerationDefaults.from_dir(src.path) if src.path and os.path.isdir(src.path) else \
         GenerationDefaults()
