@@ -22,8 +22,6 @@
 // are bf16 ones on q and p split into two bf16 parts (16 bits).
 #include <cooperative_groups.h>
 
-#include <atomic>
-
 #include "kv8.cuh"
 #include "kv8_f16.cuh"
 #include "mma_frag.cuh"
@@ -34,7 +32,6 @@ namespace cg = cooperative_groups;
 namespace hx {
 
 constexpr int kKV8Warps = 4;   // warps of a CTA
-constexpr int kKV8MaxDevices = 64;
 
 template <int D>
 struct KV8Ring {
@@ -930,26 +927,22 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
 }
 
 template <int D, int NT, int CL, bool FP8>
-static cudaError_t launch_decode(AttnDecodeKV8Args a, cudaStream_t st) {
+static cudaError_t launch_decode(const AttnDecodeKV8Args& a, cudaStream_t st) {
   auto k = attn_decode_kv8_kernel<D, NT, CL, FP8>;
   const size_t smem = sizeof(DecodeKV8Smem<D, NT, CL>);
   static_assert(sizeof(DecodeKV8Smem<D, NT, CL>) <= 113 * 1024, "two CTAs of an SM share its shared memory");
   // The clusters that fit the device at once take equal runs; one more would start when the
   // others are done. (Groups of SMs that hold no whole number of clusters leave slots empty.)
-  static std::atomic<int> fit[kKV8MaxDevices];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= kKV8MaxDevices) return cudaErrorInvalidDevice;
-  int n = fit[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static KV8Once fit;
+  int n = 0;
+  const cudaError_t e = fit.get(&n, [&](int dev, int* n) {
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     if (CL == 1) {
       int per_sm = 0, sms = 0;
       e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k, kKV8Warps * 32, smem);
       if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-      n = per_sm * sms;
+      *n = per_sm * sms;
     } else {
       cudaLaunchAttribute at;
       at.id = cudaLaunchAttributeClusterDimension;
@@ -961,15 +954,13 @@ static cudaError_t launch_decode(AttnDecodeKV8Args a, cudaStream_t st) {
       cfg.dynamicSmemBytes = smem;
       cfg.attrs = &at;
       cfg.numAttrs = 1;
-      e = cudaOccupancyMaxActiveClusters(&n, k, &cfg);
+      e = cudaOccupancyMaxActiveClusters(n, k, &cfg);
     }
-    if (e != cudaSuccess) return e;
-    n = n < 1 ? 1 : n > kKV8MaxCtas / CL ? kKV8MaxCtas / CL : n;
-    fit[dev].store(n, std::memory_order_relaxed);
-  }
-  const dim3 grid((unsigned)(n * CL)), block(kKV8Warps * 32);
-  if (CL == 1) return hx_launch_pdl(k, grid, block, smem, st, a);
-  return hx_launch_pdl_cluster(k, grid, block, smem, st, CL, a);
+    *n = *n < 1 ? 1 : *n > kKV8MaxCtas / CL ? kKV8MaxCtas / CL : *n;
+    return e;
+  });
+  if (e != cudaSuccess) return e;
+  return kv8_launch(k, dim3((unsigned)(n * CL)), kKV8Warps * 32, smem, st, CL, a);
 }
 
 template <int D, int NT, bool FP8>

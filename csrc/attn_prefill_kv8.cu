@@ -628,13 +628,18 @@ static cudaError_t launch_prefill(const AttnPrefillKV8Args& a, cudaStream_t st) 
   auto k = attn_prefill_kv8_kernel<D, NT, BN, FP8>;
   const size_t smem = sizeof(PrefillKV8Smem<D, NT, BN>) + 1024;
   static_assert(sizeof(PrefillKV8Smem<D, NT, BN>) + 1024 <= 227 * 1024, "shared memory");
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static KV8Once ready;
+  int one = 0;
+  cudaError_t e = ready.get(&one, [&](int, int* one) {
+    *one = 1;
+    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  });
   if (e != cudaSuccess) return e;
   const int R = a.T * (a.Hq / a.c.Hkv);
-  e = hx_launch_pdl(k, dim3((unsigned)a.c.Hkv, (unsigned)((R + 128 * NT - 1) / (128 * NT)), (unsigned)a.splits),
-                    dim3(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 * NT), smem, st, a);
+  e = kv8_launch(k, dim3((unsigned)a.c.Hkv, (unsigned)((R + 128 * NT - 1) / (128 * NT)), (unsigned)a.splits),
+                 32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 * NT, smem, st, 1, a);
   if (e != cudaSuccess || a.splits == 1) return e;
-  return hx_launch_pdl(attn_prefill_kv8_merge<D>, dim3((unsigned)(((long long)a.c.Hkv * R + 3) / 4)), dim3(128), 0, st, a);
+  return kv8_launch(attn_prefill_kv8_merge<D>, dim3((unsigned)(((long long)a.c.Hkv * R + 3) / 4)), 128, 0, st, 1, a);
 }
 
 cudaError_t attn_prefill_kv8_launch(const AttnPrefillKV8Args& a, cudaStream_t st) {

@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -129,6 +130,49 @@ HX_DEVICE void load16(const __nv_bfloat16* row, int d0, int vec, float* f) {
   load8(row, d0, vec, f);
   load8(row, d0 + 8, vec, f + 8);
 }
+
+// Launch with programmatic stream serialization, in clusters along x if cluster > 1. The kernels here
+// have one launch shape each, so nothing is asked about them at every call (a query costs about as
+// much as the smallest kernels run).
+template <typename Args>
+inline cudaError_t kv8_launch(void (*kernel)(Args), dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster,
+                              const Args& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = hx_pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+// Work that a kernel needs once on each device (its shared-memory limit): 0 until `set` has run
+// without an error, then what `set` left there.
+constexpr int kKV8MaxDevices = 64;
+struct KV8Once {
+  std::atomic<int> at[kKV8MaxDevices];
+  template <typename F>
+  cudaError_t get(int* value, F&& set) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= kKV8MaxDevices) return cudaErrorInvalidDevice;
+    *value = at[dev].load(std::memory_order_relaxed);
+    if (*value == 0) {
+      e = set(dev, value);
+      if (e == cudaSuccess) at[dev].store(*value, std::memory_order_relaxed);
+    }
+    return e;
+  }
+};
 
 // Calls f(integral_constant<head dim>, true_type for e4m3 or false_type for int8).
 template <typename F>

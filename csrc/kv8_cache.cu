@@ -234,7 +234,7 @@ cudaError_t kv8_append_launch(const KV8AppendArgs& a, cudaStream_t st) {
   const dim3 grid((unsigned)((a.p0 + a.T - 1) / kKV8Block - a.b0 + 1), (unsigned)a.c.Hkv, 2);
   cudaError_t e = cudaSuccess;
   kv8_dispatch(a.c.D, a.c.fp8, [&](auto d, auto fp8) {
-    e = hx_launch_pdl(kv8_append_kernel<decltype(d)::value, decltype(fp8)::value>, grid, dim3(128), 0, st, a);
+    e = kv8_launch(kv8_append_kernel<decltype(d)::value, decltype(fp8)::value>, grid, 128, 0, st, 1, a);
   });
   return e;
 }
@@ -243,7 +243,7 @@ cudaError_t kv8_read_launch(const KV8ReadArgs& a, cudaStream_t st) {
   const dim3 grid((unsigned)((a.start + a.n - 1) / kKV8Block - a.start / kKV8Block + 1), (unsigned)a.c.Hkv, 2);
   cudaError_t e = cudaSuccess;
   kv8_dispatch(a.c.D, a.c.fp8, [&](auto d, auto fp8) {
-    e = hx_launch_pdl(kv8_read_kernel<decltype(d)::value, decltype(fp8)::value>, grid, dim3(128), 0, st, a);
+    e = kv8_launch(kv8_read_kernel<decltype(d)::value, decltype(fp8)::value>, grid, 128, 0, st, 1, a);
   });
   return e;
 }
