@@ -373,8 +373,8 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
     const int u0 = unit - part;  // the pair's first unit
     // The part with the last block has more to do there; it gets fewer of the others.
     const int heavy = cuts > 1 ? min(12, s->chunk / 4) : 0;
-    const int blk0 = (int)((long long)part * (nb + heavy) / cuts);
-    const int blk1 = part + 1 == cuts ? nb : (int)((long long)(part + 1) * (nb + heavy) / cuts);
+    const int blk0 = (int)((unsigned)(part * (nb + heavy)) / (unsigned)cuts);  // (below 2^31: 320 parts, 2^22 blocks)
+    const int blk1 = part + 1 == cuts ? nb : (int)((unsigned)((part + 1) * (nb + heavy)) / (unsigned)cuts);
     const int pair = b * PB + pl, h = HG == 1 ? pl : pl / HG, hg = pl - h * HG, g0 = hg * per, n = min(per, G - g0);
     const int slot = s->slot[b], p = s->pos[b], row = p % kKV8Block;
     const __nv_bfloat16* pr = a.proj + b * a.ldp;
@@ -448,6 +448,8 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       }
     }
     if (!(completes && warp == host)) fill();
+    const int half = a.rot / 2;
+    if (tid < half) rotation((float)(p + delta) * freq, &s->sn[tid], &s->cs[tid]);
     // ---- q of the group's heads (and the new key): norm, rotation ------------------------------
     // Rows go over D / 8 lanes each, 8 dims to a lane.
     auto row_max = [](auto x) {
@@ -480,9 +482,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       }
     }
     if (cta_last && rr == 0) *reinterpret_cast<uint4*>(s->vnew + d0) = vx;
-    const int half = a.rot / 2;
     if (half) {
-      if (tid < half) rotation((float)(p + delta) * freq, &s->sn[tid], &s->cs[tid]);
       __syncthreads();
 #pragma unroll 1
       for (int r = warp; r < nrow; r += NW) {
@@ -820,27 +820,40 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
       *reinterpret_cast<float4*>(&s->wo[0][r][d]) = O;  // this thread alone reads and writes them
       if (d == 0) { s->cm[r] = M; s->cl[r] = L; }
     }
-    // ---- merge the cluster's CTAs: each finishes 1 / CL of the columns -------------------
+    // ---- merge the cluster's CTAs: each finishes 1 / CL of the columns (four dims of a head) --------
+    constexpr int MC = (GP * (D / 4) / CL + NTH - 1) / NTH;  // most columns of a thread
+    const int cols = n * (D / 4) / CL, c0 = crank * cols;
+    uint2 gate[MC];  // under way meanwhile
+#pragma unroll
+    for (int c = 0; c < MC; ++c) {
+      const int i = c0 + c * NTH + tid;
+      if (!a.gated || c * NTH + tid >= cols) continue;
+      const __nv_bfloat16* gp = pr + (long long)(h * G + g0 + i / (D / 4)) * qw + D + i % (D / 4) * 4;
+      if (a.vec) {
+        gate[c] = *reinterpret_cast<const uint2*>(gp);
+      } else {
+        const unsigned short* u = reinterpret_cast<const unsigned short*>(gp);
+        gate[c] = make_uint2(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16);
+      }
+    }
     all_sync();
-    auto finish = [&](int r, int d, float4 o, float l) {  // four dims of the output
-      const int hq = h * G + g0 + r;
+    auto finish = [&](int i, float4 o, float l, uint2 gv) {  // column i of the output
       const float il = __fdividef(1.f, l);
       float f[4] = {o.x * il, o.y * il, o.z * il, o.w * il};
       if (a.gated) {
-        const __nv_bfloat16* gp = pr + (long long)hq * qw + D + d;
+        const float x[4] = {__uint_as_float(gv.x << 16), __uint_as_float(gv.x & 0xffff0000u),
+                            __uint_as_float(gv.y << 16), __uint_as_float(gv.y & 0xffff0000u)};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = __fdividef(f[e], 1.f + __expf(-__bfloat162float(gp[e])));
+        for (int e = 0; e < 4; ++e) f[e] = __fdividef(f[e], 1.f + __expf(-x[e]));
       }
-      uint2 y;
-      y.x = pack_bf16x2(f[0], f[1]);
-      y.y = pack_bf16x2(f[2], f[3]);
-      *reinterpret_cast<uint2*>(a.out + ((long long)b * a.Hq + hq) * D + d) = y;
+      reinterpret_cast<uint2*>(a.out + ((long long)b * a.Hq + h * G + g0) * D)[i] =
+          make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
     };
     const bool alone = cuts == 1;
-    const int cols = n * (D / 4) / CL, c0 = crank * cols;  // in fours
-#pragma unroll 1
-    for (int i = c0 + tid; i < c0 + cols; i += NTH) {
-      const int r = i / (D / 4), d = i % (D / 4) * 4;
+#pragma unroll
+    for (int c = 0; c < MC; ++c) {
+      if (c * NTH + tid >= cols) continue;
+      const int i = c0 + c * NTH + tid, r = i / (D / 4), d = i % (D / 4) * 4;
       float m[CL], l[CL], M = -INFINITY, L = 0.f;
       float4 v[CL], O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -858,67 +871,75 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
         add4(O, v[x], f);
       }
       if (alone) {
-        finish(r, d, O, L);
+        finish(i, O, L, gate[c]);
       } else {
         reinterpret_cast<float4*>(part_o + (long long)unit * (GP * D))[i] = O;
         if (d == 0) part_ml[(long long)unit * GP + r] = make_float2(M, L);
       }
     }
-    if (!alone) __threadfence();
     tc::fence_proxy_async_smem();  // O's stores before the next unit's copies into the same memory
     all_sync();
     if (!alone) {
-      // the CTA or cluster that finishes the last of the pair's units merges their partials
+      // The CTA or cluster that finishes the last of the pair's units merges their partials. The
+      // barrier before and the atomic's order (release, then acquire) make every unit's visible.
       if (crank == 0 && tid == 0) {
         int* counter = a.ws + kKV8Err + pair;
-        const int last = atomicAdd(counter, 1) == cuts - 1;
+        int before;
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+        const int last = before == cuts - 1;
         if (last) *counter = 0;
-        __threadfence();
         for (int x = 0; x < CL; ++x) *peer(&s->last, x) = last;
       }
       all_sync();
       if (s->last) {
-        __threadfence();
-        const int np = cuts;
-        const long long q0 = u0;
-        const int r0 = c0 / (D / 4), r1 = (c0 + cols - 1) / (D / 4);       // heads of this CTA's columns
+        const float4* po = reinterpret_cast<const float4*>(part_o + (long long)u0 * (GP * D));
+        auto load = [&](int x0, float4 (&v)[MC][8]) {  // eight partials of every column, all under way
+#pragma unroll
+          for (int c = 0; c < MC; ++c)
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              v[c][x] = c * NTH + tid < cols && x0 + x < cuts
+                            ? __ldcg(po + (long long)(x0 + x) * (GP * D / 4) + c0 + c * NTH + tid)
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        float4 v[MC][8];
+        load(0, v);
+        const int r0 = c0 / (D / 4), r1 = (c0 + cols - 1) / (D / 4);  // heads of this CTA's columns
 #pragma unroll 1
         for (int r = r0 + warp; r <= r1; r += NW) {
-          constexpr int NX = (SM::kMaxPart + 31) / 32;
-          float2 ml[NX];
           float M = -INFINITY, L = 0.f;
-#pragma unroll
-          for (int x = 0; x < NX; ++x)
-            ml[x] = x * 32 + lane < np ? __ldcg(&part_ml[(q0 + x * 32 + lane) * GP + r]) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-          for (int x = 0; x < NX; ++x) M = fmaxf(M, ml[x].x);
+#pragma unroll 1
+          for (int x = lane; x < cuts; x += 32) M = fmaxf(M, __ldcg(&part_ml[(long long)(u0 + x) * GP + r].x));
           M = warp_max(M);
-#pragma unroll
-          for (int x = 0; x < NX; ++x) {
-            const float f = ml[x].x == -INFINITY ? 0.f : exp2_fast(ml[x].x - M);
-            if (x * 32 + lane < np) s->fw[r][x * 32 + lane] = f;
-            L = fmaf(ml[x].y, f, L);
+#pragma unroll 1
+          for (int x = lane; x < cuts; x += 32) {
+            const float2 ml = __ldcg(&part_ml[(long long)(u0 + x) * GP + r]);
+            const float f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - M);
+            s->fw[r][x] = f;
+            L = fmaf(ml.y, f, L);
           }
           L = warp_sum(L);
           if (lane == 0) s->lsum[r] = L;
         }
         __syncthreads();
-#pragma unroll 1
-        for (int i = c0 + tid; i < c0 + cols; i += NTH) {
-          const int r = i / (D / 4), d = i % (D / 4) * 4;
-          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-          for (int x = 0; x < np; x += 16) {  // sixteen loads in flight
-            float4 v[16];
+        float4 O[MC];
 #pragma unroll
-            for (int y = 0; y < 16; ++y)
-              v[y] = x + y < np ? __ldcg(reinterpret_cast<const float4*>(part_o + (q0 + x + y) * (GP * D)) + i)
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < MC; ++c) O[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int x0 = 0;;) {
 #pragma unroll
-            for (int y = 0; y < 16; ++y) add4(O, v[y], x + y < np ? s->fw[r][x + y] : 0.f);
+          for (int c = 0; c < MC; ++c) {
+            const float* fw = s->fw[min((c0 + c * NTH + tid) / (D / 4), GP - 1)] + x0;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) add4(O[c], v[c][x], x0 + x < cuts ? fw[x] : 0.f);
           }
-          finish(r, d, O, s->lsum[r]);
+          x0 += 8;
+          if (x0 >= cuts) break;
+          load(x0, v);
         }
+#pragma unroll
+        for (int c = 0; c < MC; ++c)
+          if (c * NTH + tid < cols) finish(c0 + c * NTH + tid, O[c], s->lsum[(c0 + c * NTH + tid) / (D / 4)], gate[c]);
         tc::fence_proxy_async_smem();  // the weights lie in the ring's memory
         __syncthreads();
       }

@@ -25,7 +25,7 @@ static KV8 kv8_args(const torch::Tensor& kc, const torch::Tensor& vc, const torc
   TORCH_CHECK(kc.scalar_type() == at::kChar || kv8_is_fp8(kc), "cache codes are int8 or float8_e4m3fn");
   const int64_t S = kc.size(0), H = kc.size(1), nb = kc.size(2), n = kc.size(3);
   TORCH_CHECK(n == 1 || n == 2 || n == 4, "head dim 64, 128 or 256");
-  TORCH_CHECK(S >= 1 && H >= 1 && nb >= 1 && nb <= (1 << 24), "empty cache, or more than 2^29 tokens");
+  TORCH_CHECK(S >= 1 && H >= 1 && nb >= 1 && nb <= (1 << 22), "empty cache, or more than 2^27 tokens");
   TORCH_CHECK(vc.scalar_type() == kc.scalar_type() && vc.is_contiguous() && vc.sizes() == at::IntArrayRef({S, H, nb, n, 64, kKV8Block}),
               "vc [S, Hkv, NB, D/64, 64, 32] like kc");
   for (const auto& t : {ks, vs})
