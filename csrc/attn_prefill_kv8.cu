@@ -131,7 +131,7 @@ struct PrefillKV8Smem {
   float vinv[SC][BN / 32];
   float red[3][16];
   float tail[4];                        // K tail: up, down; V tail: up, down
-  uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], sc_full[SC], s_full[2], p_full[2], o_done[NT];
+  uint64_t q_full, k_full[ST], k_empty[ST], v_full[ST], v_empty[ST], sc_full[SC], s_full[2], p_half[2], p_full[2], o_done[NT];
   uint32_t tmem_base;
   int abort;
 };
@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&s->s_full[i], 1);
+      tc::mbar_init(&s->p_half[i], 4);
       tc::mbar_init(&s->p_full[i], 4);
     }
     for (int i = 0; i < SC; ++i) tc::mbar_init(&s->sc_full[i], 1);
@@ -176,6 +177,22 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
   }
   pdl_wait_prior();
   pdl_launch_dependents();
+  // ---- the softmax warps' first rows of q, under way while the scales are looked at --------------
+  constexpr int LR = D / 8, RI = 32 / LR;  // lanes of a row of q, 8 dims each; rows of a warp's step
+  const int su = (warp - CW) >> 2, sq = warp & 3;            // row tile, TMEM lane quarter
+  const int srow = sq * 32 + lane, sr = r0 + su * 128 + srow;  // a softmax thread's row
+  const bool soft = warp >= CW && warp < MMA_WARP, live = soft && sr < R;
+  const int t = live ? sr / G : a.T - 1, hq = h * G + (live ? sr % G : 0);
+  const long long qoff = live ? t * a.ldq + (long long)hq * D : -1;
+  uint4 qx[8];
+  auto load_q = [&](int b) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const long long off = __shfl_sync(0xffffffffu, qoff, (b + k) * RI + lane / LR);
+      qx[k] = off >= 0 ? load8_raw(a.q + off, lane % LR * 8, a.vec_q) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  if (soft) load_q(0);
   // ---- the largest V scale in sight, and the tail's scales ---------------------------------------
   const uint8_t* kc = a.c.kc + a.c.block(a.slot, h, 0) * (D * kKV8Block);
   const uint8_t* vc = a.c.vc + a.c.block(a.slot, h, 0) * (D * kKV8Block);
@@ -370,15 +387,25 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
       auto pv = [&](int i) {
         const int j = i / NT, u = i % NT, st = j % ST;
         if (u == 0 && !wait(&s->v_full[st], (j / ST) & 1, 7005)) return false;
-        if (!wait(&s->p_full[i & 1], (i >> 1) & 1, 7006)) return false;
+        if (BN == 128 && !wait(&s->p_half[i & 1], (i >> 1) & 1, 7006)) return false;
         tc::tc_fence_after();
         const uint64_t v0 = vd + st * (BN * D * 2 / 16);
         const uint32_t d = tm + u * D, p = tm + S_COL + (i & 1) * BN;
         const uint32_t more = j > 0 ? 1u : 0u;
-        if (elect_one()) {
+        // P of 128 keys comes in halves: the first one's product runs while the softmax is at the second
+        auto half = [&](int k0) {
 #pragma unroll
-          for (int k = 0; k < BN / 16; ++k)
+          for (int k = k0; k < k0 + 4; ++k)
             umma_f16_ts(d, p + k * 8, v0 + (k >> 2) * (D * 128 / 16) + (k & 3) * 2, id_o, k > 0 ? 1u : more);
+        };
+        if (BN == 128) {
+          if (elect_one()) half(0);
+          __syncwarp();
+        }
+        if (!wait(&s->p_full[i & 1], (i >> 1) & 1, 7011)) return false;
+        tc::tc_fence_after();
+        if (elect_one()) {
+          half(BN / 16 - 4);
           tc::umma_commit(&s->o_done[u]);
           if (u == NT - 1) tc::umma_commit(&s->v_empty[st]);
         }
@@ -395,32 +422,24 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
     }
   } else {
     // ------------------------------------ softmax ------------------------------------------------
-    const int q = warp & 3;              // TMEM lane quarter of this warp
-    const int u = (warp - CW) >> 2;      // tile
-    const int row = q * 32 + lane, r = r0 + u * 128 + row;
-    const bool live = r < R;
-    const int t = live ? r / G : a.T - 1, hq = h * G + (live ? r % G : 0), pos = a.p0 + t;
+    const int q = sq, u = su, row = srow, r = sr, pos = a.p0 + t;
     const uint32_t lane_at = (uint32_t)(q * 32) << 16;
     // The warp brings in its 32 rows, 8 dims to a lane and RI rows at a time; lane i keeps row i's
     // score factor.
     float qs = 0.f;
     {
-      constexpr int LR = D / 8, RI = 32 / LR;
       const int ld = lane % LR, lr = lane / LR;  // 8 dims from 8 ld of row lr of a step
-      const long long mine = live ? t * a.ldq + (long long)hq * D : -1;  // lane i: row i
       unsigned char* base = reinterpret_cast<unsigned char*>(s->Q[u]) + (ld >> 3) * (128 * 128) + q * 32 * 128;
 #pragma unroll 1
       for (int b = 0; b < LR; b += 8) {
         uint4 x[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const long long off = __shfl_sync(0xffffffffu, mine, (b + k) * RI + lr);
-          x[k] = off >= 0 ? load8_raw(a.q + off, ld * 8, a.vec_q) : make_uint4(0u, 0u, 0u, 0u);
-        }
+        for (int k = 0; k < 8; ++k) x[k] = qx[k];
+        if (b + 8 < LR) load_q(b + 8);
         uint32_t mx[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          mx[k] = kv8_max2_finite(kv8_max2_finite(kv8_max2_finite(kv8_max2_finite(0u, x[k].x), x[k].y), x[k].z), x[k].w);
+          mx[k] = kv8_max2(kv8_max2(kv8_max2(kv8_max2(0u, x[k].x), x[k].y), x[k].z), x[k].w);
           mx[k] = max(mx[k] & 0xffffu, mx[k] >> 16);
         }
 #pragma unroll
@@ -540,6 +559,12 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
           l = fmaf(sum, s->vinv[j % SC][c * 2 + g], l);
         }
         tmem_st32(sa + c * 32, y);  // over scores that this thread has read twice
+        if (c + 1 < BN / 64) {
+          tmem_wait_st();
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&s->p_half[sl]);
+        }
       }
       tmem_wait_st();
       tc::tc_fence_before();
