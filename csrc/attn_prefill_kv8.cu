@@ -92,6 +92,29 @@ HX_DEVICE constexpr uint32_t idesc_f16_f32(int M, int N) {
   return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);  // f32 accumulator, f16 A and B
 }
 
+// The larger of three; two products or sums at once.
+HX_DEVICE float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+HX_DEVICE float2 fma2(float2 a, float2 b, float2 c) {
+  float2 y;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return y;
+}
+HX_DEVICE float2 add2(float2 a, float2 b) {
+  float2 y;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n"
+      " mov.b64 {%0, %1}, d;\n}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return y;
+}
+
 // A power of two that takes a largest magnitude to 128..256, and its inverse (zero stays as it is).
 HX_DEVICE void pow2_scale(float mag, float* up, float* down) {
   const int ex = min(134 - (int)(__float_as_uint(mag) >> 23), 120);
@@ -510,7 +533,7 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
         for (int g = 0; g < 2; ++g) {
           float y = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) y = fmaxf(y, x[g * 32 + e]);
+          for (int e = 0; e < 32; e += 2) y = max3(y, x[g * 32 + e], x[g * 32 + e + 1]);
           mx = fmaxf(mx, y * km[c * 2 + g]);
         }
       }
@@ -548,15 +571,16 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           const float b = s->vadd[j % SC][c * 2 + g] - base;
-          float sum = 0.f;
+          const float2 f2 = make_float2(km[c * 2 + g], km[c * 2 + g]), b2 = make_float2(b, b);
+          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float p0 = exp2_fast(fmaf(x[g * 32 + e], km[c * 2 + g], b));
-            const float p1 = exp2_fast(fmaf(x[g * 32 + e + 1], km[c * 2 + g], b));
-            sum += p0 + p1;
-            y[g * 16 + e / 2] = pack_f16x2(p0, p1);
+            const float2 z = fma2(make_float2(x[g * 32 + e], x[g * 32 + e + 1]), f2, b2);
+            const float2 p = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+            sum = add2(sum, p);
+            y[g * 16 + e / 2] = pack_f16x2(p.x, p.y);
           }
-          l = fmaf(sum, s->vinv[j % SC][c * 2 + g], l);
+          l = fmaf(sum.x + sum.y, s->vinv[j % SC][c * 2 + g], l);
         }
         tmem_st32(sa + c * 32, y);  // over scores that this thread has read twice
         if (c + 1 < BN / 64) {
