@@ -134,6 +134,9 @@ torch::Tensor kv8_workspace(int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
                       torch::TensorOptions().dtype(torch::kInt).device(torch::kCUDA, at::cuda::current_device()));
 }
 
+// One new token for each of B sequences (arguments as attn_decode): slots int32 [B] with tokens at
+// pos[slot], int32 [S], both on the device. Sequences of a call have slots of their own, or bring the
+// same row (padding).
 void attn_decode_kv8(torch::Tensor proj, c10::optional<torch::Tensor> q_norm_w, c10::optional<torch::Tensor> k_norm_w,
                      torch::Tensor inv_freq, torch::Tensor kc, torch::Tensor vc, torch::Tensor ks, torch::Tensor vs,
                      torch::Tensor kt, torch::Tensor vt, torch::Tensor slots, torch::Tensor pos, torch::Tensor ws,
@@ -243,7 +246,7 @@ void attn_prefill_kv8(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torch
   // Two row tiles a CTA where there are rows for them (at head dim 256 TMEM holds one), and CTAs
   // for every SM: with fewer the keys are split, at least four key tiles to a part.
   const int64_t R = T * (Hq / Hkv);
-  TORCH_CHECK(R < (1ll << 31), "T * query heads of a kv head past 2^31");
+  TORCH_CHECK(R <= 65535 * 128, "T * query heads of a kv head past 8388480");  // rows of the grid
   a.NT = D <= 128 && R > 128 ? 2 : 1;
   const int64_t ctas = (R + 128 * a.NT - 1) / (128 * a.NT) * Hkv;
   const int sms = at::cuda::getDeviceProperties(kc.device().index())->multiProcessorCount;

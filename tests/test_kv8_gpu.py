@@ -290,6 +290,9 @@ PREFILL = [
     (513, 700, 64, 8, 2, False),
     (1030, 7, 128, 8, 2, False),
     (9, 3000, 128, 32, 8, False),
+    (3, 2500, 256, 4, 1, True),     # keys split over CTAs at head dim 256
+    (1, 5000, 64, 2, 2, False),
+    (40, 4100, 128, 8, 1, True),    # split, two row tiles
 ]
 
 
@@ -312,6 +315,90 @@ def test_attn_prefill_kv8(fmt, T, p0, D, Hq, H, gated):
         o = o * torch.sigmoid(torch.stack([gate[:, 2 * D * h:2 * D * h + D] for h in range(Hq)], 1).double())
     _check(out[:, :Hq * D].view(T, Hq, D), o, float(vr.abs().max()))
     assert bool(out[:, Hq * D:].isnan().all())
+
+
+@pytest.mark.parametrize("D,gated", [(64, True), (128, False), (256, True)])
+def test_unaligned_operands_give_the_same_bits(D, gated):
+    """Projections, queries, gates and outputs that start on odd elements or have odd row strides."""
+    C = _C()
+    torch.manual_seed(D)
+    H, G, B = 2, 4, 2
+    Hq, qw = H * G, 2 * D if gated else D
+    inv = 1e4 ** (-torch.arange(0, D, 2, device="cuda").float() / D)
+    wide = torch.randn(B, Hq * qw + 2 * H * D + 7, device="cuda").bfloat16()
+    outs = []
+    for proj in (wide[:, 3:3 + Hq * qw + 2 * H * D], wide[:, 3:3 + Hq * qw + 2 * H * D].contiguous()):
+        cache, _ = _filled(B, H, D, "int8", [300, 63], seed=5)
+        pos = torch.tensor([300, 63], dtype=torch.int32, device="cuda")
+        out = torch.empty(B, Hq * D, dtype=torch.bfloat16, device="cuda")
+        C.attn_decode_kv8(proj, None, None, inv, *cache, torch.arange(B, dtype=torch.int32, device="cuda"), pos,
+                          C.kv8_workspace(B, Hq, H, D), out, Hq, D, gated, 1e-6)
+        outs.append([out, *cache])
+    for x, y in zip(*outs):
+        assert torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
+    T = 37
+    cache, _ = _filled(1, H, D, "fp8", [T + 100], seed=6)
+    q = torch.randn(T, Hq * D + 5, device="cuda").bfloat16()[:, 1:1 + Hq * D]
+    gate = torch.randn(T, Hq * 2 * D + 3, device="cuda").bfloat16()[:, 3:] if gated else None
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    a = torch.empty(T, Hq * D + 9, dtype=torch.bfloat16, device="cuda")[:, 5:5 + Hq * D]
+    b = torch.empty(T, Hq * D, dtype=torch.bfloat16, device="cuda")
+    C.attn_prefill_kv8(q, *cache, 0, 100, a, Hq, D ** -0.5, gate, 2 * D, err)
+    C.attn_prefill_kv8(q.contiguous(), *cache, 0, 100, b, Hq, D ** -0.5, gate.contiguous() if gated else None, 2 * D, err)
+    assert int(err) == 0 and torch.equal(a, b)
+
+
+def test_offsets_past_32_bits():
+    """The second slot of a cache whose slots are 4.6 GB each, and positions at its far end."""
+    C = _C()
+    torch.manual_seed(2)
+    H, D, nb = 1, 128, 1_100_000
+    cache = [torch.zeros(2, H, nb, 2, BLK, 64, dtype=torch.int8, device="cuda"),
+             torch.zeros(2, H, nb, 2, 64, BLK, dtype=torch.int8, device="cuda"),
+             torch.zeros(2, H, nb, device="cuda"), torch.zeros(2, H, nb, device="cuda"),
+             torch.zeros(2, H, 2, BLK, 64, dtype=torch.bfloat16, device="cuda"),
+             torch.zeros(2, H, 2, 64, BLK, dtype=torch.bfloat16, device="cuda")]
+    k, v = torch.randn(2, 70, H, D, device="cuda").bfloat16()
+    q = torch.randn(5, 4 * D, device="cuda").bfloat16()
+    ko, vo = torch.empty(2, H, 70, D, dtype=torch.bfloat16, device="cuda")
+    for p0 in (0, nb * BLK - 96):
+        C.kv8_append(k, v, *cache, 1, p0)
+        C.kv8_read(*cache, 1, p0 + 70, p0, ko, vo)
+        kr, vr = _model(k, "int8")[0], _model(v, "int8")[0]
+        assert torch.equal(ko, kr.float().bfloat16()) and torch.equal(vo, vr.float().bfloat16())
+        if p0:
+            continue
+        out, err = torch.empty(5, 4 * D, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+        C.attn_prefill_kv8(q, *cache, 1, 65, out, 4, D ** -0.5, None, 0, err)
+        _check(out.view(5, 4, D), _attend(q.double().view(5, 4, D), kr, vr, 65, D ** -0.5), float(vr.abs().max()))
+        proj = torch.cat([q[:1], k[69:70].view(1, D), v[69:70].view(1, D)], 1)
+        o = torch.empty(1, 4 * D, dtype=torch.bfloat16, device="cuda")
+        C.attn_decode_kv8(proj, None, None, torch.ones(1, device="cuda"), *cache,
+                          torch.ones(1, dtype=torch.int32, device="cuda"), torch.tensor([0, 69], dtype=torch.int32, device="cuda"),
+                          C.kv8_workspace(1, 4, H, D), o, 4, 0, False, 1e-6)
+        _check(o.view(4, D), _attend(q[:1].double().view(1, 4, D), kr, vr, 69, D ** -0.5)[0], float(vr.abs().max()))
+    assert not cache[0][0].any()
+
+
+def test_workspace_serves_every_batch_it_was_made_for():
+    """One scratch for 48 sequences, then one, then 48: counters and partials keep apart."""
+    C = _C()
+    H, G, D = 2, 2, 64
+    lens = [700 + 40 * i for i in range(48)]
+    cache, rows = _filled(48, H, D, "int8", lens, extra=2)
+    pos = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ws = C.kv8_workspace(48, H * G, H, D)
+    proj = torch.randn(48, (H * G + 2 * H) * D, device="cuda").bfloat16()
+    inv = torch.ones(1, device="cuda")
+
+    def step(at, ws):
+        out = torch.empty(len(at), H * G * D, dtype=torch.bfloat16, device="cuda")
+        C.attn_decode_kv8(proj[at], None, None, inv, *cache, torch.tensor(at, dtype=torch.int32, device="cuda"), pos, ws,
+                          out, H * G, 0, False, 1e-6)
+        return out
+    for at in (list(range(48)), [5], [47, 3], list(range(48)), [0]):
+        assert torch.equal(step(at, ws), step(at, C.kv8_workspace(len(at), H * G, H, D))), at
+    assert int(ws[0]) == 0
 
 
 def test_decode_extreme_values():
@@ -415,6 +502,10 @@ def test_refusals():
     but(15, 129)
     but(15, 130)
     bad(C.kv8_workspace, 0, 4, 2, 128)
+    bad(C.kv8_workspace, 257, 4, 2, 128)
+    big = torch.zeros(3, 8 * D, dtype=torch.bfloat16, device="cuda")
+    bad(C.attn_decode_kv8, big, None, None, inv, *cache, torch.zeros(3, dtype=torch.int32, device="cuda"), pos, ws[:-1],
+        torch.zeros(3, 4 * D, dtype=torch.bfloat16, device="cuda"), 4, 128, False, 1e-6)
     bad(C.kv8_workspace, 1, 3, 2, 128)
     bad(C.kv8_workspace, 1, 4, 2, 96)
     C.kv8_append(k[:0], k[:0], *cache, 0, 0)                   # nothing to do
