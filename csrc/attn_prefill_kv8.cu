@@ -21,6 +21,12 @@
 //   last warp        issues the MMAs from one thread. Score buffers alternate (the two tiles', or
 //                    two of one tile), so the tensor cores work on one while the other is in softmax.
 // With few rows the keys are split over CTAs and their (O, max, sum) merged by a second kernel.
+//
+// Bound by the chain softmax -> P V -> Q K of a row tile (about 4600 cycles for 128 keys at head dim
+// 128, of which the softmax takes 2600): a prompt of 4096 tokens, 32 / 8 heads of 128, int8, takes 205
+// us (670 TFLOP/s), 8192 tokens behind 8192, 16 / 2 heads of 256, e4m3, 2.32 ms (710 TFLOP/s); 61
+// tokens behind 30007 59 us. 128-key tiles for two row tiles: with 64 keys a second score buffer fits,
+// but the MMAs' issue and waits double (239 us against 221 at the time).
 // Every wait is bounded (error code 7000 + site); on expiry the CTA stops and frees its TMEM.
 #include <cuda_fp16.h>
 

@@ -243,15 +243,23 @@ void attn_prefill_kv8(torch::Tensor q, torch::Tensor kc, torch::Tensor vc, torch
   a.vec_o = aligned(a.o, T > 1 ? a.ldo : 0);
   a.vec_g = gate && aligned(a.gate, T > 1 ? a.ldg_t : 0) && a.ldg_h % 8 == 0;
   a.err = err.data_ptr<int>();
-  // Two row tiles a CTA where there are rows for them (at head dim 256 TMEM holds one), and CTAs
-  // for every SM: with fewer the keys are split, at least four key tiles to a part.
+  // CTAs for every SM: where rows give fewer, the keys are split, at least four tiles of 128 to a part
+  // (a part costs about 6 us to start and 2.4 us a tile). Two row tiles a CTA share each converted K /
+  // V tile (4096 tokens, 32 / 8 heads: 205 us against 265 with one; 61 tokens behind 30007: 60 against
+  // 74), unless that leaves over a quarter of the SMs idle (200 tokens behind 13, 64 / 8 heads: 27
+  // against 19; 100 behind 400: 29 against 22). At head dim 256 TMEM holds one.
   const int64_t R = T * (Hq / Hkv);
   TORCH_CHECK(R <= 65535 * 128, "T * query heads of a kv head past 8388480");  // rows of the grid
-  a.NT = D <= 128 && R > 128 ? 2 : 1;
-  const int64_t ctas = (R + 128 * a.NT - 1) / (128 * a.NT) * Hkv;
   const int sms = at::cuda::getDeviceProperties(kc.device().index())->multiProcessorCount;
   const int64_t tiles = (p0 + T + 127) / 128;
-  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / ctas, tiles / 4, 32}));
+  int64_t ctas = 0;
+  auto shape = [&](int nt) {
+    ctas = (R + 128 * nt - 1) / (128 * nt) * Hkv;
+    a.NT = nt;
+    a.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / ctas, tiles / 4, 32}));
+  };
+  shape(D <= 128 && R > 128 ? 2 : 1);
+  if (a.NT == 2 && ctas * a.splits * 4 < 3 * sms) shape(1);
   torch::Tensor part;
   if (a.splits > 1) {
     part = torch::empty({a.splits * Hkv * R * (D + 2)}, ks.options());
