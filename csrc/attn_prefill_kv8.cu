@@ -128,24 +128,6 @@ HX_DEVICE void pow2_scale(float mag, float* up, float* down) {
   *down = __uint_as_float((uint32_t)(127 - ex) << 23);
 }
 
-// Gate and store 16 dims from d0 of a row.
-HX_DEVICE void finish16(const AttnPrefillKV8Args& a, int t, int hq, int d0, float* o) {
-  if (a.gate) {
-    float g[16];
-    load16(a.gate + t * a.ldg_t + hq * a.ldg_h, d0, a.vec_g, g);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[e] = __fdividef(o[e], 1.f + __expf(-g[e]));
-  }
-  __nv_bfloat16* dst = a.o + t * a.ldo + (long long)hq * (a.c.D) + d0;
-  if (a.vec_o) {
-    reinterpret_cast<bf16x8*>(dst)[0] = pack8(o);
-    reinterpret_cast<bf16x8*>(dst)[1] = pack8(o + 8);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) dst[e] = __float2bfloat16(o[e]);
-  }
-}
-
 template <int D, int NT, int BN>
 struct PrefillKV8Smem {
   static constexpr int CW = NT == 1 ? 8 : 4;  // converter warps
@@ -169,6 +151,7 @@ template <int D, int NT, int BN, bool FP8>
 __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 * NT, 1) attn_prefill_kv8_kernel(AttnPrefillKV8Args a) {
   static_assert(NT * D + 2 * BN <= 512, "TMEM: the tiles' O and two score buffers");
   using SM = PrefillKV8Smem<D, NT, BN>;
+  static_assert(sizeof(SM::K) >= NT * 4 * 8192, "the epilogue's staging");
   constexpr int CW = SM::CW, MMA_WARP = CW + 4 * NT, NTH = 32 * (MMA_WARP + 1), NG = BN / 32, NP = D / 64;
   constexpr uint32_t S_COL = NT * D, Q_COL = S_COL + 2 * BN;
   constexpr int ST = SM::ST, SC = SM::SC;
@@ -231,16 +214,22 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
   const __nv_bfloat16* vt = a.c.vt + a.c.head(a.slot, h) * (D * kKV8Block);
   const int tl = kend > nf * kKV8Block ? L - nf * kKV8Block : 0;  // tail rows that this CTA reads
   {
-    float mv = 0.f, mk = 0.f, mt = 0.f;
+    float mv = 0.f;
+    uint32_t k2 = 0u, v2 = 0u;  // maxima of packed pairs
     for (int i = tid; i < min(nf, (kend + kKV8Block - 1) / kKV8Block); i += NTH) mv = fmaxf(mv, vs[i]);
     if (tl)
-      for (int i = tid; i < D * kKV8Block; i += NTH) {
-        if (i % kKV8Panel / 64 < tl) mk = fmaxf(mk, kv8_mag(__bfloat162float(kt[i])));
-        if (i % kKV8Block < tl) mt = fmaxf(mt, kv8_mag(__bfloat162float(vt[i])));
+      for (int i = tid; i < D * kKV8Block / 8; i += NTH) {  // eight values of the tail's layouts
+        const uint4 x = *reinterpret_cast<const uint4*>(kt + i * 8), y = *reinterpret_cast<const uint4*>(vt + i * 8);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        const int left = tl - i * 8 % kKV8Block;  // rows of V's eight keys that are the sequence's
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (i * 8 % kKV8Panel / 64 < tl) k2 = kv8_max2_finite(k2, xs[e]);
+          if (2 * e < left) v2 = kv8_max2_finite(v2, 2 * e + 1 < left ? ys[e] : ys[e] & 0xffffu);
+        }
       }
     mv = warp_max(mv);
-    mk = warp_max(mk);
-    mt = warp_max(mt);
+    const float mk = kv8_bits(kv8_max1(k2)), mt = kv8_bits(kv8_max1(v2));
     if (lane == 0) { s->red[0][warp] = mv; s->red[1][warp] = mk; s->red[2][warp] = mt; }
   }
   tc::tc_fence_before();
@@ -605,27 +594,58 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
     if (nb > 0) {
       if (ok && __all_sync(0xffffffffu, tc::mbar_wait(&s->o_done[u], (nb - 1) & 1, a.err, 7010))) {
         tc::tc_fence_after();
-        const float inv = l > 0.f ? vref / l : 0.f;
+        // 64 dims at a time through shared memory (K's, which the last product of scores has left), so
+        // that rows are stored, and the gate's loaded, half a warp to a row
         const bool split = gridDim.z > 1;
-        const long long pr = ((long long)blockIdx.z * a.c.Hkv + h) * R + r;
+        const float f = split ? vref : l > 0.f ? vref / l : 0.f;
+        const long long pr = ((long long)blockIdx.z * a.c.Hkv + h) * R;
+        const long long oo = live ? t * a.ldo + (long long)hq * D : -1, go = t * a.ldg_t + hq * a.ldg_h;
+        unsigned char* mem = reinterpret_cast<unsigned char*>(s->K) + (u * 4 + q) * 8192;
+        const int c4 = lane & 15;  // dims 4 c4 .. 4 c4 + 3 of the 64
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          float o[32];
-          tc::tmem_ld32(tmem + lane_at + u * D + c * 32, o);
-          if (!live) continue;
-          if (split) {
-            float4* dst = reinterpret_cast<float4*>(a.part + pr * D + c * 32);
+        for (int c = 0; c < D / 64; ++c) {
+          float o[64];
+          tmem_ld64(tmem + lane_at + u * D + c * 64, o);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              dst[e] = make_float4(o[4 * e] * vref, o[4 * e + 1] * vref, o[4 * e + 2] * vref, o[4 * e + 3] * vref);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= inv;
-            finish16(a, t, hq, c * 32, o);
-            finish16(a, t, hq, c * 32 + 16, o + 16);
+          for (int e = 0; e < 16; ++e)
+            *reinterpret_cast<float4*>(mem + lane * 256 + ((e ^ (lane & 15)) << 4)) =
+                make_float4(o[4 * e] * f, o[4 * e + 1] * f, o[4 * e + 2] * f, o[4 * e + 3] * f);
+          __syncwarp();
+#pragma unroll 4
+          for (int k = 0; k < 16; ++k) {
+            const int rw = 2 * k + (lane >> 4), d = c * 64 + c4 * 4;
+            const long long ro = __shfl_sync(0xffffffffu, oo, rw), rg = __shfl_sync(0xffffffffu, go, rw);
+            if (ro < 0) continue;
+            float4 v = *reinterpret_cast<const float4*>(mem + rw * 256 + ((c4 ^ (rw & 15)) << 4));
+            if (split) {
+              *reinterpret_cast<float4*>(a.part + (pr + r0 + u * 128 + q * 32 + rw) * D + d) = v;
+              continue;
+            }
+            if (a.gate) {
+              const __nv_bfloat16* gp = a.gate + rg + d;
+              uint2 g;
+              if (a.vec_g) {
+                g = *reinterpret_cast<const uint2*>(gp);
+              } else {
+                const unsigned short* w = reinterpret_cast<const unsigned short*>(gp);
+                g = make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
+              }
+              v.x = __fdividef(v.x, 1.f + __expf(-__uint_as_float(g.x << 16)));
+              v.y = __fdividef(v.y, 1.f + __expf(-__uint_as_float(g.x & 0xffff0000u)));
+              v.z = __fdividef(v.z, 1.f + __expf(-__uint_as_float(g.y << 16)));
+              v.w = __fdividef(v.w, 1.f + __expf(-__uint_as_float(g.y & 0xffff0000u)));
+            }
+            const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+            __nv_bfloat16* dst = a.o + ro + d;
+            if (a.vec_o) {
+              *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+            } else {
+              dst[0] = x.x; dst[1] = x.y; dst[2] = y.x; dst[3] = y.y;
+            }
           }
+          __syncwarp();
         }
-        if (split && live) reinterpret_cast<float2*>(a.part_ml)[pr] = make_float2(m, l);
+        if (split && live) reinterpret_cast<float2*>(a.part_ml)[pr + r] = make_float2(m, l);
       } else {
         ok = false;
       }
