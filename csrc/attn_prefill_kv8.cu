@@ -611,36 +611,45 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
             *reinterpret_cast<float4*>(mem + lane * 256 + ((e ^ (lane & 15)) << 4)) =
                 make_float4(o[4 * e] * f, o[4 * e + 1] * f, o[4 * e + 2] * f, o[4 * e + 3] * f);
           __syncwarp();
-#pragma unroll 4
-          for (int k = 0; k < 16; ++k) {
-            const int rw = 2 * k + (lane >> 4), d = c * 64 + c4 * 4;
-            const long long ro = __shfl_sync(0xffffffffu, oo, rw), rg = __shfl_sync(0xffffffffu, go, rw);
-            if (ro < 0) continue;
-            float4 v = *reinterpret_cast<const float4*>(mem + rw * 256 + ((c4 ^ (rw & 15)) << 4));
-            if (split) {
-              *reinterpret_cast<float4*>(a.part + (pr + r0 + u * 128 + q * 32 + rw) * D + d) = v;
-              continue;
-            }
-            if (a.gate) {
-              const __nv_bfloat16* gp = a.gate + rg + d;
-              uint2 g;
-              if (a.vec_g) {
-                g = *reinterpret_cast<const uint2*>(gp);
-              } else {
-                const unsigned short* w = reinterpret_cast<const unsigned short*>(gp);
-                g = make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
+          const int d = c * 64 + c4 * 4;
+#pragma unroll 1
+          for (int b = 0; b < 16; b += 8) {
+            uint2 g[8];
+            if (a.gate && !split) {  // eight loads under way
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const __nv_bfloat16* gp = a.gate + __shfl_sync(0xffffffffu, go, 2 * (b + k) + (lane >> 4)) + d;
+                if (a.vec_g) {
+                  g[k] = *reinterpret_cast<const uint2*>(gp);
+                } else {
+                  const unsigned short* w = reinterpret_cast<const unsigned short*>(gp);
+                  g[k] = make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
+                }
               }
-              v.x = __fdividef(v.x, 1.f + __expf(-__uint_as_float(g.x << 16)));
-              v.y = __fdividef(v.y, 1.f + __expf(-__uint_as_float(g.x & 0xffff0000u)));
-              v.z = __fdividef(v.z, 1.f + __expf(-__uint_as_float(g.y << 16)));
-              v.w = __fdividef(v.w, 1.f + __expf(-__uint_as_float(g.y & 0xffff0000u)));
             }
-            const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
-            __nv_bfloat16* dst = a.o + ro + d;
-            if (a.vec_o) {
-              *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-            } else {
-              dst[0] = x.x; dst[1] = x.y; dst[2] = y.x; dst[3] = y.y;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int rw = 2 * (b + k) + (lane >> 4);
+              const long long ro = __shfl_sync(0xffffffffu, oo, rw);
+              float4 v = *reinterpret_cast<const float4*>(mem + rw * 256 + ((c4 ^ (rw & 15)) << 4));
+              if (split) {
+                if (ro >= 0) *reinterpret_cast<float4*>(a.part + (pr + r0 + u * 128 + q * 32 + rw) * D + d) = v;
+                continue;
+              }
+              if (a.gate) {
+                v.x = __fdividef(v.x, 1.f + __expf(-__uint_as_float(g[k].x << 16)));
+                v.y = __fdividef(v.y, 1.f + __expf(-__uint_as_float(g[k].x & 0xffff0000u)));
+                v.z = __fdividef(v.z, 1.f + __expf(-__uint_as_float(g[k].y << 16)));
+                v.w = __fdividef(v.w, 1.f + __expf(-__uint_as_float(g[k].y & 0xffff0000u)));
+              }
+              const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+              __nv_bfloat16* dst = a.o + ro + d;
+              if (ro < 0) continue;
+              if (a.vec_o) {
+                *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+              } else {
+                dst[0] = x.x; dst[1] = x.y; dst[2] = y.x; dst[3] = y.y;
+              }
             }
           }
           __syncwarp();
