@@ -23,9 +23,9 @@
 // With few rows the keys are split over CTAs and their (O, max, sum) merged by a second kernel.
 //
 // Bound by the chain softmax -> P V -> Q K of a row tile (about 4600 cycles for 128 keys at head dim
-// 128, of which the softmax takes 2600): a prompt of 4096 tokens, 32 / 8 heads of 128, int8, takes 205
-// us (670 TFLOP/s), 8192 tokens behind 8192, 16 / 2 heads of 256, e4m3, 2.32 ms (710 TFLOP/s); 61
-// tokens behind 30007 59 us. 128-key tiles for two row tiles: with 64 keys a second score buffer fits,
+// 128, of which the softmax takes 2600): a prompt of 4096 tokens, 32 / 8 heads of 128, int8, takes 184
+// us (750 TFLOP/s), 8192 tokens behind 8192, 16 / 2 heads of 256, e4m3, 2.29 ms (720 TFLOP/s); 61
+// tokens behind 30007 56 us. 128-key tiles for two row tiles: with 64 keys a second score buffer fits,
 // but the MMAs' issue and waits double (239 us against 221 at the time).
 // Every wait is bounded (error code 7000 + site); on expiry the CTA stops and frees its TMEM.
 #include <cuda_fp16.h>
@@ -183,12 +183,13 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
     s->abort = 0;
     tc::fence_barrier_init();
   }
+  // TMEM is taken after the wait and before the next kernel may start: neither of two kernels that
+  // meet on an SM holds it while it waits for the other.
+  pdl_wait_prior();
   if (warp == MMA_WARP) {
     tc::tmem_alloc(&s->tmem_base, 512);
     tc::tmem_relinquish();
   }
-  pdl_wait_prior();
-  pdl_launch_dependents();
   // ---- the softmax warps' first rows of q, under way while the scales are looked at --------------
   constexpr int LR = D / 8, RI = 32 / LR;  // lanes of a row of q, 8 dims each; rows of a warp's step
   const int su = (warp - CW) >> 2, sq = warp & 3;            // row tile, TMEM lane quarter
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(32 + 32 * PrefillKV8Smem<D, NT, BN>::CW + 128 
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
+  pdl_launch_dependents();
   float vref = 0.f;
   {
     float mk = 0.f, mt = 0.f;
