@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
   float2* part_ml = reinterpret_cast<float2*>(part_o + (long long)(kKV8MaxCtas + a.B * PB) * GP * D);  // [units][GP]
   int put = 0, get = 0;  // ring slots of the next copy issued (lane 0) and used
   uint32_t phase = 0;    // parity of the slot to use next
-  bool ok = true;
+  bool ok = true, drained = false;
   DecodeKV8Warp<D, NT, FP8> st;
 #pragma unroll 1
   for (int unit = cid; unit < units; unit += NC) {
@@ -748,16 +748,20 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
     // ---- complete blocks -----------------------------------------------------------------------
     const float* ksp = a.c.ks + a.c.block(slot, h, 0);
     const float* vsp = a.c.vs + a.c.block(slot, h, 0);
-    auto next_unit = [&](auto&& use) {  // wait for a unit, use it, hand its slot to a later one
-      if (ok) ok = tc::mbar_wait(&s->full[warp][get], phase, a.ws, 6002);
-      ok = __all_sync(0xffffffffu, ok);
-      use(s->ring[warp][get]);
-      __syncwarp();
-      if (lane == 0 && ok && todo > 0) issue();
+    auto advance = [&] {
       if (++get == R::kSlots) {
         get = 0;
         phase ^= 1;
       }
+    };
+    auto next_unit = [&](auto&& use) {  // wait for a copy, use it, hand its slot to a later one
+      if (ok) ok = tc::mbar_wait(&s->full[warp][get], phase, a.ws, 6002);
+      ok = __all_sync(0xffffffffu, ok);
+      use(s->ring[warp][get]);  // (whatever is there once a wait ran out: the error word is set)
+      __syncwarp();
+      if (!ok) return;
+      if (lane == 0 && todo > 0) issue();
+      advance();
     };
     float ks = 0.f, vs = 0.f;
     if (mine > 0) {
@@ -787,6 +791,16 @@ __global__ void __launch_bounds__(kKV8Warps * 32, 2) attn_decode_kv8_kernel(Attn
           for (int q = 0; q < R::kUnit / kKV8Panel; ++q)
             st.pv_panel(x + q * kKV8Panel, k * (R::kUnit / kKV8Panel) + q, vs0);
         });
+    }
+    if (!ok && !drained) {  // a wait ran out: give the copies under way a last bounded wait before their memory is reused
+      // from the one that did not come to the last one issued: at least one, at most all slots
+      const int under_way = (__shfl_sync(0xffffffffu, put, 0) - get + R::kSlots - 1) % R::kSlots + 1;
+#pragma unroll 1
+      for (int i = 0; i < under_way; ++i) {
+        tc::mbar_wait(&s->full[warp][get], phase, a.ws, 6002);
+        advance();
+      }
+      drained = true;  // nothing is issued any more
     }
     // ---- merge the warps: the ring's memory holds their O now --------------------------------------
     __syncthreads();
