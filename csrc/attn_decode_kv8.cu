@@ -24,7 +24,7 @@
 // Bound by the cache's bytes where there are many: 8 ragged sequences to 16K, 32 / 8 heads of 128,
 // int8: 33.5 us for 152 MB (4.5 TB/s in all, 7.5 TB/s over the 20 us in which the CTAs stream); 8
 // sequences of 131072: 318 us (6.8 TB/s). By latency where there are few: one sequence of 8192, 16 /
-// 2 heads of 256, e4m3: 13.6 us, of which 1.7 us are the blocks.
+// 2 heads of 256, e4m3: 13.8 us, of which 1.7 us are the blocks.
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"

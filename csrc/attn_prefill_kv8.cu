@@ -23,8 +23,8 @@
 // With few rows the keys are split over CTAs and their (O, max, sum) merged by a second kernel.
 //
 // Bound by the chain softmax -> P V -> Q K of a row tile (about 4600 cycles for 128 keys at head dim
-// 128, of which the softmax takes 2600): a prompt of 4096 tokens, 32 / 8 heads of 128, int8, takes 184
-// us (750 TFLOP/s), 8192 tokens behind 8192, 16 / 2 heads of 256, e4m3, 2.29 ms (720 TFLOP/s); 61
+// 128, of which the softmax takes 2600): a prompt of 4096 tokens, 32 / 8 heads of 128, int8, takes 185
+// us (740 TFLOP/s), 8192 tokens behind 8192, 16 / 2 heads of 256, e4m3, 2.30 ms (720 TFLOP/s); 61
 // tokens behind 30007 56 us. 128-key tiles for two row tiles: with 64 keys a second score buffer fits,
 // but the MMAs' issue and waits double (239 us against 221 at the time).
 // Every wait is bounded (error code 7000 + site); on expiry the CTA stops and frees its TMEM.
